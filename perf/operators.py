@@ -1,0 +1,617 @@
+"""The policy-training operators as they are measured: cases, inputs, plain forms and 64-bit values.
+
+Three operators of a policy's training step, one file:
+
+  linear / linear_backward   y = act(x w + b) + residual, and its gradients
+  policy_loss                the clipped policy loss with a KL term and an entropy bonus, with its
+                             gradient with respect to the logits
+  adamw                      decoupled-weight-decay Adam over many tensors, moments in 32 or 8 bits
+
+`run` computes them with elementary torch operations where `own` is false and through the package's
+entry points where it is true, on what `prepare` made from the seed.
+"""
+
+import itertools
+import math
+
+import torch
+
+own = False
+
+DTYPES = {'float32': torch.float32, 'bfloat16': torch.bfloat16, 'float16': torch.float16}
+BYTES = {'float32': 4, 'bfloat16': 2, 'float16': 2}
+
+# --------------------------------------------------------------------------- #
+#  cases
+# --------------------------------------------------------------------------- #
+# Tensor lists of the AdamW cases: 'AxB' is a matrix, 'r*(...)' a repetition.
+Q_NETWORK = '8x8x4x32,32,4x4x32x64,64,3x3x64x64,64,3136x512,512,512x18,18'
+BLOCKS = '4096x512,8*(2048x2048,2048,2048x4096,4096,4096x1024,1024)'
+SMALL = '300*(97,33x31,5x7x3)'
+
+MOST_MACS = 8192 * 4096 * 16384
+MOST_LOGITS = 8192 * 65536
+MOST_PARAMS = 1 << 27
+
+
+def listed():
+  return [
+      # one observation's features through the 3136 -> 512 layer of an acting network
+      dict(name='linear_one_row', op='linear', m=1, k=3136, n=512, dtype='bfloat16',
+           activation='relu', residual=False, save=False, transposed=False, pad=0),
+      # sixteen sequences in generation, one token each, a residual branch's closing product
+      dict(name='linear_few_rows', op='linear', m=16, k=8192, n=4096, dtype='bfloat16',
+           activation='none', residual=True, save=False, transposed=True, pad=0),
+      # a large batch of tokens through a widening layer, pre-activations kept for the backward pass
+      dict(name='linear_wide', op='linear', m=8192, k=4096, n=16384, dtype='bfloat16',
+           activation='gelu', residual=False, save=True, transposed=False, pad=0),
+      # odd sizes and a row pitch that no vector load divides, with a residual
+      dict(name='linear_odd', op='linear', m=1777, k=1235, n=1001, dtype='float16',
+           activation='silu', residual=True, save=False, transposed=False, pad=1),
+      # the fc1 layer's backward pass at the learners' batch and type
+      dict(name='backward_fc1', op='linear_backward', m=32, k=3136, n=512, dtype='float32',
+           activation='relu', transposed=False, pad=0),
+      # the backward pass of a hidden layer over a batch of tokens
+      dict(name='backward_hidden', op='linear_backward', m=8192, k=4096, n=4096, dtype='bfloat16',
+           activation='gelu', transposed=False, pad=0),
+      # one learner batch over the 18 actions of the full game set: latency
+      dict(name='loss_actions', op='policy_loss', rows=32, classes=18, dtype='float32',
+           ref=False, entropy=True, masked=0.3, padded=0.0, extra=0),
+      # a rollout of many steps over few actions
+      dict(name='loss_rollout', op='policy_loss', rows=131072, classes=18, dtype='float32',
+           ref=True, entropy=True, masked=0.3, padded=0.1, extra=0),
+      # a batch of padded sequences over a large vocabulary
+      dict(name='loss_tokens', op='policy_loss', rows=8192, classes=65536, dtype='bfloat16',
+           ref=True, entropy=True, masked=0.0, padded=0.2, extra=0),
+      # the dense Q-network's parameters, every learner step: launches count
+      dict(name='adamw_network', op='adamw', tensors=Q_NETWORK, dtype='float32', bits=32,
+           max_norm=10.0, packed=False),
+      # nine hundred small tensors that lie one behind the other
+      dict(name='adamw_many_small', op='adamw', tensors=SMALL, dtype='float32', bits=32,
+           max_norm=0.0, packed=True),
+      # a large network in 16 bits with master weights and 8-bit moments
+      dict(name='adamw_large_8bit', op='adamw', tensors=BLOCKS, dtype='bfloat16', bits=8,
+           max_norm=1.0, packed=False),
+  ]
+
+
+def _log_int(rng, low, high):
+  return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+  op = rng.choice(['linear', 'linear_backward', 'policy_loss', 'adamw'])
+  dtype = rng.choice(['bfloat16', 'bfloat16', 'float16', 'float32'])
+  if op in ('linear', 'linear_backward'):
+    most = MOST_MACS // (1 if op == 'linear' else 2) // (8 if dtype == 'float32' else 1)
+    while True:
+      m, k, n = _log_int(rng, 1, 16384), _log_int(rng, 8, 8192), _log_int(rng, 8, 16384)
+      if rng.random() < 0.5:   # half of them in steps that layers are built in
+        k, n = -(-k // 64) * 64, -(-n // 64) * 64
+      if m * k * n <= most:
+        break
+    c = dict(op=op, m=m, k=k, n=n, dtype=dtype,
+             activation=rng.choice(['none', 'relu', 'gelu', 'silu']),
+             transposed=rng.random() < 0.4, pad=rng.choice([0, 0, 8, 3]))
+    if op == 'linear':
+      c.update(residual=rng.random() < 0.5, save=rng.random() < 0.4)
+    return c
+  if op == 'policy_loss':
+    while True:
+      rows, classes = _log_int(rng, 1, 200000), _log_int(rng, 2, 200000)
+      if rows * classes <= MOST_LOGITS // (2 if dtype == 'float32' else 1):
+        break
+    return dict(op=op, rows=rows, classes=classes, dtype=dtype, ref=rng.random() < 0.6,
+                entropy=rng.random() < 0.6, masked=rng.choice([0.0, 0.3]),
+                padded=rng.choice([0.0, 0.2]), extra=rng.choice([0, 0, 5]))
+  total = _log_int(rng, 1000, MOST_PARAMS // 2)
+  count = _log_int(rng, 1, 40)
+  cuts = [rng.random() ** 2 + 0.01 for _ in range(count)]
+  sizes = [max(1, int(total * u / sum(cuts))) for u in cuts]
+  return dict(op=op, tensors=','.join(str(s) for s in sizes), dtype=dtype,
+              bits=rng.choice([8, 32]), max_norm=rng.choice([0.0, 1.0]),
+              packed=rng.random() < 0.5)
+
+
+def _shapes(text):
+  """'2*(4x8,8),5' -> [(4, 8), (8,), (4, 8), (8,), (5,)]."""
+  out, rest = [], text
+  while rest:
+    star, paren = rest.find('*'), rest.find(',')
+    if star >= 0 and (paren < 0 or star < paren):
+      close = rest.index(')')
+      out += _shapes(rest[star + 2:close]) * int(rest[:star])
+      rest = rest[close + 2:]
+    else:
+      head, _, rest = rest.partition(',')
+      out.append(tuple(int(d) for d in head.split('x')))
+  return out
+
+
+# --------------------------------------------------------------------------- #
+#  inputs
+# --------------------------------------------------------------------------- #
+def _generator(seed):
+  g = torch.Generator(device='cuda')
+  g.manual_seed(1000003 * int(seed) + 17)
+  return g
+
+
+def _normal(g, shape, dtype, scale=1.0):
+  return (torch.randn(shape, generator=g, device='cuda') * scale).to(dtype)
+
+
+def _uniform(g, shape, dtype, bound):
+  return ((torch.rand(shape, generator=g, device='cuda') * 2 - 1) * bound).to(dtype)
+
+
+def _pitched(t, pad):
+  """The same matrix in rows of `pad` more elements."""
+  wide = torch.zeros(t.shape[0], t.shape[1] + pad, dtype=t.dtype, device=t.device)
+  wide[:, :t.shape[1]] = t
+  return wide[:, :t.shape[1]]
+
+
+def _prepare_linear(case, g):
+  m, k, n, dtype = case['m'], case['k'], case['n'], DTYPES[case['dtype']]
+  bound = 1.0 / math.sqrt(k)
+  w = _uniform(g, (n, k) if case['transposed'] else (k, n), dtype, bound)
+  s = {'x': _pitched(_normal(g, (m, k), dtype), case['pad']),
+       'w': w.t() if case['transposed'] else w}
+  if case['op'] == 'linear':
+    s['b'] = _uniform(g, (n,), dtype, bound)
+    s['residual'] = _normal(g, (m, n), dtype) if case['residual'] else None
+  else:
+    s['dy'] = _pitched(_normal(g, (m, n), dtype, 1.0 / m), case['pad'])
+    s['preact'] = _normal(g, (m, n), dtype) if case['activation'] != 'none' else None
+  return s
+
+
+def _prepare_loss(case, g):
+  n, v, dtype = case['rows'], case['classes'], DTYPES[case['dtype']]
+  wide = _normal(g, (n, v + case['extra']), dtype, 2.0)
+  logits = wide[:, :v]
+  rows = torch.arange(n, device='cuda')
+  actions = torch.randint(0, v, (n,), generator=g, device='cuda')
+  if case['masked']:   # actions or tokens that are not allowed, never the one that was taken
+    off = torch.rand((n, v), generator=g, device='cuda') < case['masked']
+    off[rows, actions] = False
+    logits.masked_fill_(off, -math.inf)
+    del off
+  # the taken action is a likely one, as a sample of the policy is
+  logits[rows, actions] += (3 + torch.randn(n, generator=g, device='cuda')).to(dtype)
+  logp = logits[rows, actions].float() - torch.logsumexp(logits.float(), -1)
+  noise = lambda scale: scale * torch.randn(n, generator=g, device='cuda')
+  s = {'logits': logits, 'actions': actions, 'advantages': noise(1.0),
+       'old_logp': logp + noise(0.2), 'ref_logp': logp + noise(0.3) if case['ref'] else None,
+       'weights': None}
+  if case['padded']:
+    s['weights'] = (torch.rand(n, generator=g, device='cuda') >= case['padded']).float()
+  s['config'] = dict(clip_low=0.2, clip_high=0.28, kl_coef=0.05 if case['ref'] else 0.0,
+                     entropy_coef=0.01 if case['entropy'] else 0.0)
+  return s
+
+
+STATE_BLOCK = 256    # elements to a scale of the 8-bit moments; tensors begin at a multiple of it
+STEPS_BEFORE = 100
+
+
+def _prepare_adamw(case, g):
+  shapes = _shapes(case['tensors'])
+  sizes = [math.prod(s) for s in shapes]
+  room = [-(-n // STATE_BLOCK) * STATE_BLOCK for n in sizes]
+  starts = list(itertools.accumulate(room, initial=0))[:-1]
+  at = list(itertools.accumulate(sizes, initial=0))[:-1] if case['packed'] else starts
+  total, dtype = sum(room), DTYPES[case['dtype']]
+  real = torch.zeros(total, dtype=torch.bool, device='cuda')
+  for a, n in zip(starts, sizes):
+    real[a:a + n] = True
+  # gradients of very different sizes from tensor to tensor and from element to element
+  size = torch.exp(1.5 * torch.randn(total, generator=g, device='cuda') - 7) * real
+  m = size * torch.randn(total, generator=g, device='cuda') * 0.3
+  v = size * size * torch.rand(total, generator=g, device='cuda')
+  grad = size * torch.randn(total, generator=g, device='cuda')
+  master = 0.05 * torch.randn(total, generator=g, device='cuda') * real
+  del size
+  s = {'config': dict(learning_rate=1e-3, b1=0.9, b2=0.999, eps=1e-8, weight_decay=0.1,
+                      max_global_grad_norm=case['max_norm'], state_bits=case['bits']),
+       'sizes': sizes, 'room': room, 'starts': starts, 'packed': case['packed'],
+       'decay': [len(x) > 1 for x in shapes], 'count': STEPS_BEFORE, 'seed': 11,
+       'master': None, 'place': real.nonzero()[:, 0] if case['packed'] else None}
+
+  def lay(t):
+    flat = t[real].to(dtype) if case['packed'] else t.to(dtype)
+    return flat, [flat[a:a + n].view(shape) for a, n, shape in zip(at, sizes, shapes)]
+
+  s['params_flat'], s['params'] = lay(master)
+  s['grads_flat'], s['grads'] = lay(grad)
+  if dtype != torch.float32:
+    s['master'] = master
+  if case['bits'] == 8:
+    key = _mix64(_int64(s['seed']) ^ _mix64(_int64(STEPS_BEFORE)))
+    s['m'], s['m_scale'] = _to_e4m3(m, _noise(total, key, 0))
+    s['v'], s['v_scale'] = _to_e5m3(v, _noise(total, key, 1))
+  else:
+    s['m'], s['v'] = m, v
+  if own:
+    from dqn_zoo_amd import adamw
+    opt = adamw.AdamW(s['params'], adamw.AdamWConfig(**s['config']), decay=s['decay'],
+                      seed=s['seed'])
+    opt.set_state({key: s[key] for key in ('count', 'master', 'm', 'v', 'm_scale', 'v_scale')
+                   if s.get(key) is not None})
+    s['optimizer'] = opt
+  return s
+
+
+def prepare(case, seed):
+  g = _generator(seed)
+  s = {'op': case['op'], 'activation': case.get('activation'), 'save': case.get('save', False)}
+  make = {'linear': _prepare_linear, 'linear_backward': _prepare_linear,
+          'policy_loss': _prepare_loss, 'adamw': _prepare_adamw}[case['op']]
+  s.update(make(case, g))
+  return s
+
+
+# --------------------------------------------------------------------------- #
+#  plain forms
+# --------------------------------------------------------------------------- #
+def _act(z, name):
+  if name == 'relu':
+    return torch.where(z > 0, z, torch.zeros_like(z))
+  if name == 'gelu':
+    return 0.5 * z * (1 + torch.erf(z * math.sqrt(0.5)))
+  if name == 'silu':
+    return z / (1 + torch.exp(-z))
+  return z
+
+
+def _act_slope(z, name):
+  if name == 'relu':
+    return (z > 0).to(z.dtype)
+  if name == 'gelu':
+    return (0.5 * (1 + torch.erf(z * math.sqrt(0.5)))
+            + z * torch.exp(-0.5 * z * z) * (1 / math.sqrt(2 * math.pi)))
+  s = 1 / (1 + torch.exp(-z))
+  return s * (1 + z * (1 - s))
+
+
+def _plain_linear(s):
+  dtype = s['x'].dtype
+  z = s['x'].float() @ s['w'].float() + s['b'].float()
+  y = _act(z, s['activation'])
+  if s['residual'] is not None:
+    y = y + s['residual'].float()
+  return {'y': y.to(dtype), **({'preact': z.to(dtype)} if s['save'] else {})}
+
+
+def _plain_linear_backward(s):
+  dtype = s['x'].dtype
+  dz = s['dy'].float()
+  if s['preact'] is not None:
+    dz = dz * _act_slope(s['preact'].float(), s['activation'])
+  dx = dz @ s['w'].float().t()
+  dw = s['x'].float().t() @ dz
+  return {'dx': dx.to(dtype), 'dw': dw.to(dtype), 'db': dz.sum(0).to(dtype)}
+
+
+def _plain_policy_loss(s):
+  c, logits = s['config'], s['logits']
+  x = logits.float()
+  n = x.shape[0]
+  w = s['weights'] if s['weights'] is not None else torch.ones(n, device=x.device)
+  top = x.amax(-1, keepdim=True)
+  t = x - top
+  e = torch.exp(t)
+  total = e.sum(-1, keepdim=True)
+  logp_all = t - torch.log(total)
+  p = e / total
+  logp = logp_all.gather(1, s['actions'][:, None])[:, 0]
+  p_logp = torch.where(p > 0, p * logp_all, 0.0)
+  entropy = -p_logp.sum(-1)
+  ratio = torch.exp(logp - s['old_logp'])
+  adv = s['advantages']
+  free, held = ratio * adv, torch.clamp(ratio, 1 - c['clip_low'], 1 + c['clip_high']) * adv
+  loss = -torch.minimum(free, held) - c['entropy_coef'] * entropy
+  slope = torch.where(free <= held, -free, 0.0)
+  if s['ref_logp'] is not None:
+    d = s['ref_logp'] - logp
+    loss = loss + c['kl_coef'] * (torch.exp(d) - d - 1)
+    slope = slope + c['kl_coef'] * (1 - torch.exp(d))
+  used = w != 0
+  norm = w.sum()
+  scale = torch.where(used, w / norm, 0.0)
+  grad = c['entropy_coef'] * (p_logp + p * entropy[:, None]) - slope[:, None] * p
+  rows = torch.arange(n, device=x.device)
+  grad[rows, s['actions']] += slope
+  grad = torch.where(used[:, None], grad * scale[:, None], 0.0)
+  return {'loss': torch.where(used, scale * loss, 0.0).sum(),
+          'logp': torch.where(used, logp, 0.0), 'entropy': torch.where(used, entropy, 0.0),
+          'dlogits': grad.to(logits.dtype)}
+
+
+def _int64(v):
+  v &= (1 << 64) - 1
+  return torch.tensor(v - (1 << 64) if v >> 63 else v, dtype=torch.int64, device='cuda')
+
+
+def _shift(x, bits):
+  return (x >> bits) & ((1 << (64 - bits)) - 1)
+
+
+def _mix64(x):
+  """The splitmix64 step, as the package's other counter-based draws."""
+  x = x + (0x9E3779B97F4A7C15 - (1 << 64))
+  x = (x ^ _shift(x, 30)) * (0xBF58476D1CE4E5B9 - (1 << 64))
+  x = (x ^ _shift(x, 27)) * (0x94D049BB133111EB - (1 << 64))
+  return x ^ _shift(x, 31)
+
+
+def _noise(n, key, which):
+  """16 random bits for each element: one 64-bit draw serves two elements' two moments."""
+  h = _mix64(key + torch.arange((n + 1) // 2, dtype=torch.int64, device='cuda'))
+  return torch.stack([(h >> (16 * which)) & 0xFFFF, (h >> (16 * which + 32)) & 0xFFFF],
+                     -1).reshape(-1)[:n].to(torch.int32)
+
+
+def _to_e4m3(m, noise):
+  """Sign, 4 exponent and 3 fraction bits, in units of a 256-element block's largest / 448,
+  rounded up or down at random so that the mean is kept."""
+  a = m.abs().view(-1, STATE_BLOCK)
+  top = a.amax(-1, keepdim=True)
+  top = torch.where(top < 2.0 ** -118, 0.0, top)
+  y = torch.clamp(a * torch.where(top > 0, 448.0 / top, 0.0), max=448.0).reshape(-1)
+  code = ((y.view(torch.int32) + (noise << 4)) >> 20) - 960
+  small = torch.floor(y * 512.0 + noise.float() * 2.0 ** -16).to(torch.int32)
+  code = torch.where(y < 2.0 ** -6, small, code)
+  code = torch.where(m < 0, code + 128, code)
+  return code.to(torch.uint8), (top / 448.0).reshape(-1)
+
+
+def _from_e4m3(code, scale):
+  return (code.view(torch.float8_e4m3fn).float().view(-1, STATE_BLOCK) * scale[:, None]).reshape(-1)
+
+
+def _to_e5m3(v, noise):
+  """5 exponent and 3 fraction bits, no sign, in units of a block's largest / 1.875; what is not
+  zero stays so."""
+  a = v.view(-1, STATE_BLOCK)
+  top = a.amax(-1, keepdim=True)
+  top = torch.where(top < 2.0 ** -118, 0.0, top)
+  y = torch.clamp(a * torch.where(top > 0, 1.875 / top, 0.0), max=1.875).reshape(-1)
+  code = ((y.view(torch.int32) + (noise << 4)) >> 20) - 768
+  small = torch.floor(y * 2.0 ** 33 + noise.float() * 2.0 ** -16).to(torch.int32)
+  code = torch.where(y < 2.0 ** -30, small, code)
+  code = torch.where((y > 0) & (code == 0), 1, code)
+  return code.to(torch.uint8), (top / 1.875).reshape(-1)
+
+
+def _from_e5m3(code, scale):
+  c = code.to(torch.int32)
+  y = torch.where(c < 8, c.float() * 2.0 ** -33, ((c + 768) << 20).view(torch.float32))
+  return (y.view(-1, STATE_BLOCK) * scale[:, None]).reshape(-1)
+
+
+def _plain_adamw(s):
+  c = s['config']
+  dtype, count = s['params_flat'].dtype, s['count'] + 1
+  s['count'] = count
+
+  def gather(flat):
+    if not s['packed']:
+      return flat.float()
+    return torch.zeros(sum(s['room']), device='cuda').index_copy_(0, s['place'], flat.float())
+
+  g = gather(s['grads_flat'])
+  norm = torch.sqrt((g * g).sum())
+  if c['max_global_grad_norm'] > 0:
+    g = g * torch.where(norm < c['max_global_grad_norm'], 1.0, c['max_global_grad_norm'] / norm)
+  p = s['master'] if s['master'] is not None else gather(s['params_flat'])
+  eight = c['state_bits'] == 8
+  m = _from_e4m3(s['m'], s['m_scale']) if eight else s['m']
+  v = _from_e5m3(s['v'], s['v_scale']) if eight else s['v']
+  m = c['b1'] * m + (1 - c['b1']) * g
+  v = c['b2'] * v + (1 - c['b2']) * (g * g)
+  wd = torch.tensor([c['weight_decay'] if d else 0.0 for d in s['decay']], device='cuda')
+  wd = torch.repeat_interleave(wd, torch.tensor(s['room'], device='cuda'))
+  step = (m / (1 - c['b1'] ** count)) / (torch.sqrt(v / (1 - c['b2'] ** count)) + c['eps'])
+  p = p - c['learning_rate'] * (step + wd * p)
+  if s['master'] is not None:
+    s['master'] = p
+  s['params_flat'].copy_(p[s['place']] if s['packed'] else p)
+  if eight:
+    key = _mix64(_int64(s['seed']) ^ _mix64(_int64(count)))
+    s['m'], s['m_scale'] = _to_e4m3(m, _noise(m.numel(), key, 0))
+    s['v'], s['v_scale'] = _to_e5m3(v, _noise(v.numel(), key, 1))
+    m, v = _from_e4m3(s['m'], s['m_scale']), _from_e5m3(s['v'], s['v_scale'])
+    # neighbouring 8-bit values are 1/15 apart or more: 16 bits tell them apart
+    m, v = m.to(torch.bfloat16), v.to(torch.bfloat16)
+  else:
+    s['m'], s['v'] = m, v
+  out = {'params': s['params_flat'], 'm': m, 'v': v}
+  if dtype != torch.float32:
+    out['master'] = s['master']
+  if c['max_global_grad_norm'] > 0:
+    out['norm'] = norm
+  return out
+
+
+# --------------------------------------------------------------------------- #
+#  the package's calls
+# --------------------------------------------------------------------------- #
+def _own_linear(s):
+  from dqn_zoo_amd import linear
+  y = linear.linear(s['x'], s['w'], s['b'], activation=s['activation'], residual=s['residual'],
+                    save_preact=s['save'])
+  return {'y': y[0], 'preact': y[1]} if s['save'] else {'y': y}
+
+
+def _own_linear_backward(s):
+  from dqn_zoo_amd import linear
+  dx, dw, db = linear.linear_backward(s['dy'], s['x'], s['w'], activation=s['activation'],
+                                      preact=s['preact'])
+  return {'dx': dx, 'dw': dw, 'db': db}
+
+
+def _own_policy_loss(s):
+  from dqn_zoo_amd import policy_loss
+  out = policy_loss.policy_loss(
+      s['logits'], s['actions'], s['advantages'], s['old_logp'], ref_logp=s['ref_logp'],
+      weights=s['weights'], config=policy_loss.PolicyLossConfig(**s['config']))
+  return {'loss': out.loss, 'logp': out.logp, 'entropy': out.entropy, 'dlogits': out.dlogits}
+
+
+def _own_adamw(s):
+  opt = s['optimizer']
+  opt.step(s['grads'])
+  m, v = opt.moments(torch.bfloat16) if s['config']['state_bits'] == 8 else (opt.m, opt.v)
+  out = {'params': s['params_flat'], 'm': m, 'v': v}
+  if s['master'] is not None:
+    out['master'] = opt.master
+  if s['config']['max_global_grad_norm'] > 0:
+    out['norm'] = opt.grad_norm
+  return out
+
+
+def run(state):
+  if own:
+    return {'linear': _own_linear, 'linear_backward': _own_linear_backward,
+            'policy_loss': _own_policy_loss, 'adamw': _own_adamw}[state['op']](state)
+  return {'linear': _plain_linear, 'linear_backward': _plain_linear_backward,
+          'policy_loss': _plain_policy_loss, 'adamw': _plain_adamw}[state['op']](state)
+
+
+# --------------------------------------------------------------------------- #
+#  work of one pass, and its values in 64 bits
+# --------------------------------------------------------------------------- #
+def work(case):
+  if case['op'] in ('linear', 'linear_backward'):
+    m, k, n, b = case['m'], case['k'], case['n'], BYTES[case['dtype']]
+    if case['op'] == 'linear':
+      moved = m * k + k * n + n + m * n * (1 + case['residual'] + case['save'])
+      return {'bytes': b * moved, 'flops': 2 * m * k * n}
+    moved = m * n * (2 if case['activation'] != 'none' else 1) + 2 * (m * k + k * n) + n
+    return {'bytes': b * moved, 'flops': 4 * m * k * n}
+  if case['op'] == 'policy_loss':
+    n, v = case['rows'], case['classes']
+    rows = 8 + 4 * (4 + case['ref'] + (case['padded'] > 0))
+    used = 1 - case['padded']   # a row without weight is written, and not read
+    return {'bytes': n * v * BYTES[case['dtype']] * (1 + used) + n * rows, 'flops': 12 * n * v}
+  n = sum(math.prod(s) for s in _shapes(case['tensors']))
+  b = BYTES[case['dtype']]
+  moments = 16 if case['bits'] == 32 else 4 + 4   # read and written; the 8-bit ones also given out
+  weights = 2 * b if case['dtype'] == 'float32' else 8 + b
+  return {'bytes': n * (weights + b + moments), 'flops': 20 * n}
+
+
+def _exact_linear(case, s):
+  x, w = s['x'].double(), s['w'].double()
+  name = case['activation']
+  gauss = torch.distributions.Normal(torch.zeros((), dtype=torch.float64, device='cuda'), 1.0)
+  if case['op'] == 'linear':
+    z = torch.addmm(s['b'].double()[None, :].expand(x.shape[0], -1), x, w)
+    y = {'none': lambda: z, 'relu': lambda: z.clamp(min=0), 'gelu': lambda: z * gauss.cdf(z),
+         'silu': lambda: z * torch.sigmoid(z)}[name]()
+    y = y if s['residual'] is None else y + s['residual'].double()
+    return {'y': y, 'preact': z} if case['save'] else {'y': y}
+  dz = s['dy'].double()
+  if name != 'none':
+    z = s['preact'].double()
+    if name == 'relu':
+      dz = dz.masked_fill(z <= 0, 0.0)
+    elif name == 'gelu':
+      dz = dz * (gauss.cdf(z) + z * gauss.log_prob(z).exp())
+    else:
+      dz = dz * (torch.sigmoid(z) + z * torch.sigmoid(z) * torch.sigmoid(-z))
+  return {'dx': torch.mm(dz, w.t()), 'dw': torch.mm(x.t(), dz), 'db': dz.sum(0)}
+
+
+def _exact_loss(case, s):
+  c, n = s['config'], case['rows']
+  w = torch.ones(n, device='cuda') if s['weights'] is None else s['weights']
+  w = w.double()
+  total, out = w.sum(), []
+  for rows in torch.arange(n, device='cuda').split(max(1, (1 << 27) // case['classes'])):
+    lp = torch.log_softmax(s['logits'][rows].double(), -1)
+    a = s['actions'][rows][:, None]
+    logp = lp.gather(1, a).squeeze(1)
+    plp = torch.special.entr(lp.exp())
+    h = plp.sum(-1)
+    adv = s['advantages'][rows].double()
+    ratio = (logp - s['old_logp'][rows].double()).exp()
+    low, high = 1 - c['clip_low'], 1 + c['clip_high']
+    inside = torch.where(adv >= 0, ratio <= high, ratio >= low)
+    kept = torch.where(adv >= 0, ratio.clamp(max=high), ratio.clamp(min=low))
+    value, pull = -kept * adv - c['entropy_coef'] * h, -ratio * adv * inside
+    if s['ref_logp'] is not None:
+      d = s['ref_logp'][rows].double() - logp
+      value, pull = value + c['kl_coef'] * (d.expm1() - d), pull - c['kl_coef'] * d.expm1()
+    u = (w[rows] / total)
+    grad = -(pull[:, None] * lp.exp()) + c['entropy_coef'] * (lp.exp() * h[:, None] - plp)
+    grad = grad.scatter_add(1, a, pull[:, None]) * u[:, None]
+    live = w[rows] != 0
+    zero = torch.zeros((), dtype=torch.float64, device='cuda')
+    out.append((torch.where(live, u * value, zero), torch.where(live, logp, zero),
+                torch.where(live, h, zero), torch.where(live[:, None], grad, zero)))
+  value, logp, h, grad = (torch.cat(t) for t in zip(*out))
+  return {'loss': value.sum(), 'logp': logp, 'entropy': h, 'dlogits': grad}
+
+
+def _exact_eight(a, noise, top_value, least, bits):
+  """Values of a rounded to a float of 3 fraction bits and least exponent `least`, at random."""
+  a = a.view(-1, STATE_BLOCK)
+  top = a.amax(-1, keepdim=True)
+  unit = torch.where(top > 0, top / top_value, 1.0)
+  y = a / unit
+  _, exponent = torch.frexp(y)
+  step = torch.exp2(torch.clamp(exponent.double() - 1, min=least) - 3)
+  near = torch.floor(y / step + noise.view(-1, STATE_BLOCK).double() / 65536) * step
+  if bits == 'unsigned':
+    near = torch.where((y > 0) & (near == 0), 2.0 ** (least - 3), near)
+  return (near.clamp(max=top_value) * unit).reshape(-1)
+
+
+def _exact_adamw(case, s):
+  c, t = s['config'], s['count'] + 1
+  out = {'params': [], 'm': [], 'v': [], 'master': []}
+  if case['bits'] == 8:
+    m0 = s['m'].view(torch.float8_e4m3fn).double().view(-1, STATE_BLOCK) * s['m_scale'].double()[:, None]
+    code = s['v'].double()
+    v0 = torch.where(code < 8, code / 8, (1 + torch.remainder(code, 8) / 8)
+                     * torch.exp2(torch.floor(code / 8) - 1)) * 2.0 ** -30
+    v0 = v0.view(-1, STATE_BLOCK) * s['v_scale'].double()[:, None]
+    m0, v0 = m0.reshape(-1), v0.reshape(-1)
+  else:
+    m0, v0 = s['m'].double(), s['v'].double()
+  norm = s['grads_flat'].double().norm()
+  limit = c['max_global_grad_norm']
+  clip = torch.clamp(limit / norm, max=1.0) if limit > 0 else 1.0
+  for i, (a, r, n) in enumerate(zip(s['starts'], s['room'], s['sizes'])):
+    g = s['grads'][i].double().reshape(-1) * clip
+    p = s['params'][i].double().reshape(-1) if s['master'] is None else s['master'][a:a + n].double()
+    m = m0[a:a + n].lerp(g, 1 - c['b1'])
+    v = v0[a:a + n].lerp(g.square(), 1 - c['b2'])
+    q = p * (1 - c['learning_rate'] * c['weight_decay'] * s['decay'][i])
+    q = q - c['learning_rate'] / (1 - c['b1'] ** t) * m / ((v / (1 - c['b2'] ** t)).sqrt() + c['eps'])
+    wide = lambda x, r=r, n=n: torch.nn.functional.pad(x, (0, r - n))
+    for name, x in (('params', q), ('m', m), ('v', v), ('master', q)):
+      out[name].append(wide(x) if name != 'params' or not case['packed'] else x)
+  out = {name: torch.cat(parts) for name, parts in out.items()}
+  if case['bits'] == 8:
+    total = out['m'].numel()
+    key = _mix64(_int64(s['seed']) ^ _mix64(_int64(t)))
+    out['m'] = torch.sign(out['m']) * _exact_eight(out['m'].abs(), _noise(total, key, 0), 448.0, -6, 'signed')
+    out['v'] = _exact_eight(out['v'], _noise(total, key, 1), 1.875, -30, 'unsigned')
+  if s['master'] is None:
+    del out['master']
+  if limit > 0:
+    out['norm'] = norm
+  return out
+
+
+def exact(case, seed):
+  s = prepare(case, seed)
+  if case['op'] == 'policy_loss':
+    return _exact_loss(case, s)
+  if case['op'] == 'adamw':
+    return _exact_adamw(case, s)
+  return _exact_linear(case, s)
