@@ -26,6 +26,7 @@ ARCH = 'gfx950'
 CXXFLAGS = [
     '--offload-arch=' + ARCH, '-O3', '-std=c++17', '-fPIC',
     '-ffp-contract=off', '-fno-fast-math', '-Wall', '-Wno-unused-function',
+    '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
     '-I', INCLUDE,
 ]
 
