@@ -239,7 +239,7 @@ def _prepare_adamw(case, g):
                       seed=s['seed'])
     opt.set_state({key: s[key] for key in ('count', 'master', 'm', 'v', 'm_scale', 'v_scale')
                    if s.get(key) is not None})
-    s['optimizer'] = opt
+    s['optimizer'], s['bound'] = opt, opt.bind(s['grads'])   # gradient buffers that stay
   return s
 
 
@@ -462,7 +462,7 @@ def _own_policy_loss(s):
 
 def _own_adamw(s):
   opt = s['optimizer']
-  opt.step(s['grads'])
+  opt.step(s['bound'])
   m, v = opt.moments(torch.bfloat16) if s['config']['state_bits'] == 8 else (opt.m, opt.v)
   out = {'params': s['params_flat'], 'm': m, 'v': v}
   if s['master'] is not None:
