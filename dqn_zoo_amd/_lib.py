@@ -193,9 +193,29 @@ class RainbowActArgs(ctypes.Structure):
               ('greedy_out', c_vp), ('vmax_out', c_vp)]
 
 
+class AdamWTensor(ctypes.Structure):
+  """dz_adamw_tensor_t."""
+  _fields_ = [('p', c_vp), ('n', c_i64), ('offset', c_i64), ('decay', c_f32), ('reserved', c_i32)]
+
+
+class AdamWArgs(ctypes.Structure):
+  """dz_adamw_args_t."""
+  _fields_ = [('param_dtype', c_i32), ('grad_dtype', c_i32), ('state_bits', c_i32),
+              ('num_chunks', c_i32), ('tensors', c_vp), ('chunks', c_vp), ('grads', c_vp),
+              ('master', c_vp), ('m', c_vp), ('v', c_vp), ('m_scale', c_vp), ('v_scale', c_vp),
+              ('count', c_vp), ('lr', c_vp), ('scalars', c_vp), ('partials', c_vp),
+              ('b1', c_f64), ('b2', c_f64), ('eps', c_f32), ('max_norm', c_f32),
+              ('grad_scale', c_f32), ('reserved', c_i32), ('seed', ctypes.c_uint64)]
+
+
+# element types of the size-generic operators (DZ_F32 / DZ_BF16 / DZ_F16)
+F32, BF16, F16 = 0, 1, 2
+ADAMW_STATE_BLOCK, ADAMW_CHUNK = 256, 4096
+
 STRUCT_IDS = {0: FieldDesc, 1: PrioSampleArgs, 2: RainbowLayout, 3: RainbowArgs,
               4: DenseLayout, 5: DenseArgs, 6: IqnLayout, 7: IqnArgs,
-              8: InsertField, 9: NextSample, 10: ReplayInsertArgs, 11: RainbowActArgs}
+              8: InsertField, 9: NextSample, 10: ReplayInsertArgs, 11: RainbowActArgs,
+              12: AdamWTensor, 13: AdamWArgs}
 
 # name -> (restype, argtypes).  tests/test_abi.py checks this table against
 # the prototypes in include/dqnzoo_hip.h and against the built library.
@@ -271,6 +291,9 @@ SIGNATURES = {
     'dz_prioritized_update': (c_int, [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp,
                                       c_vp, c_int, c_f64, c_int, c_vp, c_vp,
                                       c_vp]),
+    'dz_adamw_bind': (c_int, [c_vp, c_int, c_vp, c_vp]),
+    'dz_adamw_step': (c_int, [ctypes.POINTER(AdamWArgs), c_vp]),
+    'dz_adamw_moments': (c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_vp]),
     'dz_prioritized_add': (c_int, [c_vp, c_i64, c_i64, c_i64, c_int, c_f64,
                                    c_vp, c_f64, c_vp, c_vp]),
 }
@@ -368,6 +391,50 @@ def ptr(t):
   if t is None:
     return None
   return t.data_ptr()
+
+
+_dtype_codes = {}
+
+
+def dtype_code(dtype):
+  """DZ_F32 / DZ_BF16 / DZ_F16 of a torch dtype; None for any other."""
+  if not _dtype_codes:
+    import torch
+    _dtype_codes.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+  return _dtype_codes.get(dtype)
+
+
+def gpu_index(name, t):
+  """The device index of a GPU tensor; a TypeError or HipLibraryError for anything else (there
+  is no CPU path)."""
+  import torch
+  if not isinstance(t, torch.Tensor):
+    raise TypeError('%s must be a tensor, got %s' % (name, type(t).__name__))
+  if not t.is_cuda:
+    raise HipLibraryError('%s is on %s: the operators run on an AMD GPU; no CPU fallback' %
+                          (name, t.device))
+  return t.get_device()
+
+
+class _NoGuard:
+
+  def __enter__(self):
+    return self
+
+  def __exit__(self, *exc):
+    return False
+
+
+_no_guard = _NoGuard()
+
+
+def device_guard(index):
+  """Makes `index` the current device for a `with` block (free if it already is): launches go to
+  the tensors' device, whichever is current."""
+  import torch
+  if torch.cuda.current_device() == index:
+    return _no_guard
+  return torch.cuda.device(index)
 
 
 def current_stream_ptr():

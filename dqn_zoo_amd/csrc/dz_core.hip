@@ -30,6 +30,8 @@ extern "C" int dz_struct_size(int which) {
     case 9: return (int)sizeof(dz_next_sample_t);
     case 10: return (int)sizeof(dz_replay_insert_args_t);
     case 11: return (int)sizeof(dz_rainbow_act_args_t);
+    case 12: return (int)sizeof(dz_adamw_tensor_t);
+    case 13: return (int)sizeof(dz_adamw_args_t);
     default: return -1;
   }
 }

@@ -56,7 +56,8 @@ const char* dz_built_arch(void);
  * can verify its mirror: 0 dz_field_t, 1 dz_prio_sample_args_t,
  * 2 dz_rainbow_layout_t, 3 dz_rainbow_args_t, 4 dz_dense_layout_t, 9 dz_next_sample_t,
  * 5 dz_dense_args_t, 6 dz_iqn_layout_t, 7 dz_iqn_args_t, 8 dz_insert_field_t,
- * 10 dz_replay_insert_args_t, 11 dz_rainbow_act_args_t.
+ * 10 dz_replay_insert_args_t, 11 dz_rainbow_act_args_t, 12 dz_adamw_tensor_t,
+ * 13 dz_adamw_args_t.
  * -1 for an unknown id.                                                      */
 int dz_struct_size(int which);
 
@@ -754,6 +755,71 @@ int dz_atari_observation(const uint8_t* const* frames, int n_frames, int height,
  *  - dz_rainbow_layout: batch <= 1024.
  * There are no run-time tuning knobs: launch shapes are compile-time constants
  * (csrc/dz_rainbow.hip, csrc/dz_qnet_kernels.h), chosen by measurement.       */
+
+/* ------------------------------------------------------------------------- *
+ *  Operators of a policy's training step, for any size and three element types.
+ *  The reference trains Q-networks only and has no counterpart of these.
+ *  Sizes are elements, strides are elements; rows are `ld*` elements apart and
+ *  their elements adjacent.  Arithmetic is float32 (sums that span rows: float64
+ *  where noted); each result is rounded once, to the element type of its buffer.
+ * ------------------------------------------------------------------------- */
+#define DZ_F32 0
+#define DZ_BF16 1
+#define DZ_F16 2
+
+/* AdamW (decoupled weight decay) over a list of tensors in one launch
+ * (csrc/dz_adamw.hip):
+ *   g = grad * grad_scale * min(1, max_norm / (grad_scale * |all gradients|))
+ *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+ *   p = p - lr ((m / bc1) / (sqrt(v / bc2) + eps) + decay p),  bcX = 1 - bX^step
+ * The moments (and the float32 master copy of 16-bit parameters) live in flat
+ * buffers in which every tensor begins at a multiple of DZ_ADAMW_STATE_BLOCK.
+ * state_bits 32: float32.  state_bits 8: one byte per element and one float32
+ * scale per DZ_ADAMW_STATE_BLOCK elements; m as OCP e4m3, v as an unsigned float
+ * of 5 exponent and 3 fraction bits (code c >= 8: (1 + (c & 7)/8) 2^((c >> 3) - 31),
+ * c < 8: c 2^-33), both rounded at random (counter-based, keyed by seed and step).
+ * A gradient that is not finite makes the parameters it meets NaN.              */
+#define DZ_ADAMW_STATE_BLOCK 256
+#define DZ_ADAMW_CHUNK 4096
+typedef struct {
+  void* p;             /* contiguous, element type param_dtype, any alignment the type allows */
+  int64_t n;           /* elements, > 0                                          */
+  int64_t offset;      /* of its state in the flat buffers, a multiple of DZ_ADAMW_STATE_BLOCK */
+  float decay;         /* its weight decay                                       */
+  int32_t reserved;
+} dz_adamw_tensor_t;
+
+typedef struct {
+  int32_t param_dtype;       /* DZ_F32 / DZ_BF16 / DZ_F16                        */
+  int32_t grad_dtype;        /* param_dtype or DZ_F32                            */
+  int32_t state_bits;        /* 32 or 8                                          */
+  int32_t num_chunks;
+  const dz_adamw_tensor_t* tensors;   /* device                                  */
+  const int32_t* chunks;     /* device [num_chunks][2]: tensor, DZ_ADAMW_CHUNK-element piece of it */
+  const void* const* grads;  /* device table of the gradients' pointers (dz_adamw_bind) */
+  float* master;             /* flat float32 master weights, or NULL (float32 parameters: NULL) */
+  void* m;
+  void* v;
+  float* m_scale;            /* state_bits 8 only                                */
+  float* v_scale;
+  int32_t* count;            /* steps done; incremented                          */
+  const float* lr;           /* device, so that a captured step follows a schedule */
+  float* scalars;            /* 8 words: [0] the scaled gradients' norm (0 without clipping), [1..5] internal */
+  float* partials;           /* num_chunks words; NULL without clipping          */
+  double b1, b2;
+  float eps, max_norm;       /* max_norm <= 0: no clipping, no norm              */
+  float grad_scale;
+  int32_t reserved;
+  uint64_t seed;
+} dz_adamw_args_t;
+
+/* table[i] = grads[i] (host array of device pointers), as kernels: capturable. */
+int dz_adamw_bind(const void* const* grads, int num_tensors, const void** table, dz_stream_t stream);
+int dz_adamw_step(const dz_adamw_args_t* args, dz_stream_t stream);
+/* The 8-bit moments as numbers of type dtype, [count] each (count a multiple of
+ * DZ_ADAMW_STATE_BLOCK).                                                       */
+int dz_adamw_moments(const uint8_t* m, const uint8_t* v, const float* m_scale, const float* v_scale,
+                     int64_t count, int dtype, void* m_out, void* v_out, dz_stream_t stream);
 
 /* dst = src for a parameter buffer (target network sync,
  * ref: rainbow/agent.py:157-158).                                           */
