@@ -208,6 +208,17 @@ class AdamWArgs(ctypes.Structure):
               ('grad_scale', c_f32), ('reserved', c_i32), ('seed', ctypes.c_uint64)]
 
 
+class PolicyLossArgs(ctypes.Structure):
+  """dz_policy_loss_args_t."""
+  _fields_ = [('dtype', c_i32), ('reserved', c_i32), ('rows', c_i64), ('classes', c_i64),
+              ('logits', c_vp), ('ld', c_i64), ('actions', c_vp), ('advantages', c_vp),
+              ('old_logp', c_vp), ('ref_logp', c_vp), ('weights', c_vp), ('dlogits', c_vp),
+              ('ldg', c_i64), ('loss', c_vp), ('logp', c_vp), ('entropy', c_vp),
+              ('status', c_vp), ('ws', c_vp), ('ws_bytes', c_i64), ('clip_low', c_f64),
+              ('clip_high', c_f64), ('normalizer', c_f64), ('kl_coef', c_f32),
+              ('entropy_coef', c_f32), ('grad_scale', c_f32), ('reserved2', c_i32)]
+
+
 # element types of the size-generic operators (DZ_F32 / DZ_BF16 / DZ_F16)
 F32, BF16, F16 = 0, 1, 2
 ADAMW_STATE_BLOCK, ADAMW_CHUNK = 256, 4096
@@ -215,7 +226,7 @@ ADAMW_STATE_BLOCK, ADAMW_CHUNK = 256, 4096
 STRUCT_IDS = {0: FieldDesc, 1: PrioSampleArgs, 2: RainbowLayout, 3: RainbowArgs,
               4: DenseLayout, 5: DenseArgs, 6: IqnLayout, 7: IqnArgs,
               8: InsertField, 9: NextSample, 10: ReplayInsertArgs, 11: RainbowActArgs,
-              12: AdamWTensor, 13: AdamWArgs}
+              12: AdamWTensor, 13: AdamWArgs, 14: PolicyLossArgs}
 
 # name -> (restype, argtypes).  tests/test_abi.py checks this table against
 # the prototypes in include/dqnzoo_hip.h and against the built library.
@@ -294,6 +305,8 @@ SIGNATURES = {
     'dz_adamw_bind': (c_int, [c_vp, c_int, c_vp, c_vp]),
     'dz_adamw_step': (c_int, [ctypes.POINTER(AdamWArgs), c_vp]),
     'dz_adamw_moments': (c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_vp]),
+    'dz_policy_loss_workspace': (c_int, [c_int, c_i64, c_i64, ctypes.POINTER(c_i64)]),
+    'dz_policy_loss': (c_int, [ctypes.POINTER(PolicyLossArgs), c_vp]),
     'dz_prioritized_add': (c_int, [c_vp, c_i64, c_i64, c_i64, c_int, c_f64,
                                    c_vp, c_f64, c_vp, c_vp]),
 }
@@ -375,13 +388,17 @@ def capture_graph(stream, enqueue):
                        '`torch.cuda.stream(torch.cuda.Stream())`')
   # (refused -- ValueError -- while the event profiler is on: its marks are
   # event records between the kernels and cannot live inside a graph)
+  global _raw_capture
   check(lib.dz_graph_capture_begin(stream), 'dz_graph_capture_begin')
   h = ctypes.c_void_p()
+  _raw_capture = True
   try:
     enqueue()
   except BaseException:
     lib.dz_graph_capture_end(stream, 1, ctypes.byref(h))
     raise
+  finally:
+    _raw_capture = False
   check(lib.dz_graph_capture_end(stream, 0, ctypes.byref(h)), 'dz_graph_capture_end')
   return h
 
@@ -414,6 +431,38 @@ def gpu_index(name, t):
     raise HipLibraryError('%s is on %s: the operators run on an AMD GPU; no CPU fallback' %
                           (name, t.device))
   return t.get_device()
+
+
+# set while `capture_graph` records: torch's allocator does not know of such a capture, and would
+# hand memory that the graph uses to somebody else
+_raw_capture = False
+
+
+def scratch(nbytes, device_index, workspace):
+  """An operator's workspace: the caller's `workspace` (a contiguous uint8 tensor, checked) or a
+  block of torch's allocator on the current stream."""
+  import torch
+  if workspace is None:
+    if _raw_capture:
+      raise RuntimeError('inside capture_graph the operators need the caller\'s workspace= and '
+                         'output buffers: they must live as long as the graph')
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=torch.device('cuda', device_index))
+  if gpu_index('workspace', workspace) != device_index:
+    raise ValueError('workspace is on another device')
+  if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+    raise TypeError('workspace must be a contiguous uint8 tensor')
+  if workspace.numel() < nbytes or workspace.data_ptr() % 16:
+    raise ValueError('workspace needs %d bytes, 16-byte aligned; got %d' % (nbytes, workspace.numel()))
+  return workspace
+
+
+def new_output(shape, dtype, device):
+  """torch.empty, refused inside capture_graph (see `scratch`)."""
+  import torch
+  if _raw_capture:
+    raise RuntimeError('inside capture_graph the operators need the caller\'s workspace= and '
+                       'output buffers: they must live as long as the graph')
+  return torch.empty(shape, dtype=dtype, device=device)
 
 
 class _NoGuard:

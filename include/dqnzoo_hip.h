@@ -57,7 +57,7 @@ const char* dz_built_arch(void);
  * 2 dz_rainbow_layout_t, 3 dz_rainbow_args_t, 4 dz_dense_layout_t, 9 dz_next_sample_t,
  * 5 dz_dense_args_t, 6 dz_iqn_layout_t, 7 dz_iqn_args_t, 8 dz_insert_field_t,
  * 10 dz_replay_insert_args_t, 11 dz_rainbow_act_args_t, 12 dz_adamw_tensor_t,
- * 13 dz_adamw_args_t.
+ * 13 dz_adamw_args_t, 14 dz_policy_loss_args_t.
  * -1 for an unknown id.                                                      */
 int dz_struct_size(int which);
 
@@ -820,6 +820,41 @@ int dz_adamw_step(const dz_adamw_args_t* args, dz_stream_t stream);
  * DZ_ADAMW_STATE_BLOCK).                                                       */
 int dz_adamw_moments(const uint8_t* m, const uint8_t* v, const float* m_scale, const float* v_scale,
                      int64_t count, int dtype, void* m_out, void* v_out, dz_stream_t stream);
+
+/* The clipped policy loss with a KL term and an entropy bonus, and its gradient
+ * (csrc/dz_policy_loss.hip).  Row i: log-softmax of logits[i], rho = exp(logp - old_logp),
+ *   value = -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A)
+ *           + kl_coef (exp(d) - d - 1) - entropy_coef H,        d = ref_logp - logp
+ *   loss = sum_i weights[i] value[i] / norm
+ * norm: `normalizer`, or the sum of the weights (the number of rows without weights) where
+ * that is 0.  dlogits = grad_scale * d loss / d logits, rounded once; it may be the logits'
+ * own buffer (same pointer and pitch).  A row of weight 0 is not looked at (its action may
+ * be anything): logp, entropy and gradient 0.  An action outside [0, classes) makes its row
+ * and the loss NaN and sets DZ_ST_BAD_INDEX in `status`.  A row whose logits are all -inf,
+ * or hold NaN or +inf, is NaN.  All weights 0: loss and gradient 0.                      */
+typedef struct {
+  int32_t dtype;             /* of logits and dlogits                            */
+  int32_t reserved;
+  int64_t rows, classes;     /* classes < 2^30, rows < 2^31                      */
+  const void* logits; int64_t ld;
+  const int64_t* actions;    /* [rows]                                           */
+  const float* advantages;
+  const float* old_logp;
+  const float* ref_logp;     /* or NULL: no KL term                              */
+  const float* weights;      /* or NULL: all 1                                   */
+  void* dlogits; int64_t ldg;  /* or NULL: values only                           */
+  float* loss;               /* [1]                                              */
+  float* logp;               /* [rows]                                           */
+  float* entropy;            /* [rows]                                           */
+  uint32_t* status;          /* or NULL                                          */
+  void* ws; int64_t ws_bytes;  /* dz_policy_loss_workspace; 16-byte aligned, contents arbitrary */
+  double clip_low, clip_high, normalizer;
+  float kl_coef, entropy_coef, grad_scale;
+  int32_t reserved2;
+} dz_policy_loss_args_t;
+
+int dz_policy_loss_workspace(int dtype, int64_t rows, int64_t classes, int64_t* bytes);
+int dz_policy_loss(const dz_policy_loss_args_t* args, dz_stream_t stream);
 
 /* dst = src for a parameter buffer (target network sync,
  * ref: rainbow/agent.py:157-158).                                           */
