@@ -219,6 +219,17 @@ class PolicyLossArgs(ctypes.Structure):
               ('entropy_coef', c_f32), ('grad_scale', c_f32), ('reserved2', c_i32)]
 
 
+class LinearArgs(ctypes.Structure):
+  """dz_linear_args_t."""
+  _fields_ = [('dtype', c_i32), ('activation', c_i32), ('m', c_i64), ('k', c_i64), ('n', c_i64),
+              ('x', c_vp), ('ldx', c_i64), ('w', c_vp), ('ldw', c_i64), ('w_transposed', c_i32),
+              ('bias_f32', c_i32), ('bias', c_vp), ('residual', c_vp), ('ldr', c_i64),
+              ('y', c_vp), ('ldy', c_i64), ('preact', c_vp), ('ldz', c_i64), ('dy', c_vp),
+              ('lddy', c_i64), ('dx', c_vp), ('lddx', c_i64), ('dw', c_vp), ('lddw', c_i64),
+              ('db', c_vp), ('grads_f32', c_i32), ('reserved', c_i32), ('ws', c_vp),
+              ('ws_bytes', c_i64)]
+
+
 # element types of the size-generic operators (DZ_F32 / DZ_BF16 / DZ_F16)
 F32, BF16, F16 = 0, 1, 2
 ADAMW_STATE_BLOCK, ADAMW_CHUNK = 256, 4096
@@ -226,7 +237,8 @@ ADAMW_STATE_BLOCK, ADAMW_CHUNK = 256, 4096
 STRUCT_IDS = {0: FieldDesc, 1: PrioSampleArgs, 2: RainbowLayout, 3: RainbowArgs,
               4: DenseLayout, 5: DenseArgs, 6: IqnLayout, 7: IqnArgs,
               8: InsertField, 9: NextSample, 10: ReplayInsertArgs, 11: RainbowActArgs,
-              12: AdamWTensor, 13: AdamWArgs, 14: PolicyLossArgs}
+              12: AdamWTensor, 13: AdamWArgs, 14: PolicyLossArgs,
+              15: LinearArgs}
 
 # name -> (restype, argtypes).  tests/test_abi.py checks this table against
 # the prototypes in include/dqnzoo_hip.h and against the built library.
@@ -305,6 +317,9 @@ SIGNATURES = {
     'dz_adamw_bind': (c_int, [c_vp, c_int, c_vp, c_vp]),
     'dz_adamw_step': (c_int, [ctypes.POINTER(AdamWArgs), c_vp]),
     'dz_adamw_moments': (c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_vp]),
+    'dz_linear_workspace': (c_int, [ctypes.POINTER(LinearArgs), c_int, ctypes.POINTER(c_i64)]),
+    'dz_linear': (c_int, [ctypes.POINTER(LinearArgs), c_vp]),
+    'dz_linear_backward': (c_int, [ctypes.POINTER(LinearArgs), c_vp]),
     'dz_policy_loss_workspace': (c_int, [c_int, c_i64, c_i64, ctypes.POINTER(c_i64)]),
     'dz_policy_loss': (c_int, [ctypes.POINTER(PolicyLossArgs), c_vp]),
     'dz_prioritized_add': (c_int, [c_vp, c_i64, c_i64, c_i64, c_int, c_f64,

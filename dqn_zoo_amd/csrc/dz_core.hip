@@ -33,6 +33,7 @@ extern "C" int dz_struct_size(int which) {
     case 12: return (int)sizeof(dz_adamw_tensor_t);
     case 13: return (int)sizeof(dz_adamw_args_t);
     case 14: return (int)sizeof(dz_policy_loss_args_t);
+    case 15: return (int)sizeof(dz_linear_args_t);
     default: return -1;
   }
 }

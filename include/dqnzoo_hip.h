@@ -57,7 +57,7 @@ const char* dz_built_arch(void);
  * 2 dz_rainbow_layout_t, 3 dz_rainbow_args_t, 4 dz_dense_layout_t, 9 dz_next_sample_t,
  * 5 dz_dense_args_t, 6 dz_iqn_layout_t, 7 dz_iqn_args_t, 8 dz_insert_field_t,
  * 10 dz_replay_insert_args_t, 11 dz_rainbow_act_args_t, 12 dz_adamw_tensor_t,
- * 13 dz_adamw_args_t, 14 dz_policy_loss_args_t.
+ * 13 dz_adamw_args_t, 14 dz_policy_loss_args_t, 15 dz_linear_args_t.
  * -1 for an unknown id.                                                      */
 int dz_struct_size(int which);
 
@@ -820,6 +820,44 @@ int dz_adamw_step(const dz_adamw_args_t* args, dz_stream_t stream);
  * DZ_ADAMW_STATE_BLOCK).                                                       */
 int dz_adamw_moments(const uint8_t* m, const uint8_t* v, const float* m_scale, const float* v_scale,
                      int64_t count, int dtype, void* m_out, void* v_out, dz_stream_t stream);
+
+/* A dense layer with its epilogue, and its backward pass (csrc/dz_linear.hip):
+ *   z = x w + bias;  y = act(z) + residual                    x [m][k], w [k][n]
+ *   dz = dy act'(preact);  dx = dz w^T;  dw = x^T dz;  db = column sums of dz
+ * (the residual's gradient is dy).  One element type for x, w, residual, y, preact, dy,
+ * dx; float32 products and sums; dz is rounded to the element type before the two
+ * products of the backward pass (their matrix instructions take that type), not before
+ * db.  w_transposed: w (and dw) is stored [n][k].  GELU is the erf form.              */
+#define DZ_ACT_NONE 0
+#define DZ_ACT_RELU 1
+#define DZ_ACT_GELU 2
+#define DZ_ACT_SILU 3
+typedef struct {
+  int32_t dtype, activation;
+  int64_t m, k, n;           /* each 1 .. 2^31 - 1025                            */
+  const void* x; int64_t ldx;
+  const void* w; int64_t ldw;
+  int32_t w_transposed;
+  int32_t bias_f32;          /* bias is float32 whatever dtype is                */
+  const void* bias;          /* [n] or NULL                                      */
+  const void* residual; int64_t ldr;   /* [m][n] or NULL; may be y               */
+  void* y; int64_t ldy;      /* dz_linear                                        */
+  void* preact; int64_t ldz; /* z: written by dz_linear (or NULL), read by dz_linear_backward */
+  /* dz_linear_backward: */
+  const void* dy; int64_t lddy;
+  void* dx; int64_t lddx;    /* each of dx, dw, db may be NULL: not computed     */
+  void* dw; int64_t lddw;
+  void* db;
+  int32_t grads_f32;         /* dw and db are float32 whatever dtype is          */
+  int32_t reserved;
+  void* ws; int64_t ws_bytes;  /* dz_linear_workspace; 16-byte aligned, contents arbitrary */
+} dz_linear_args_t;
+
+/* Bytes of workspace for these dtype, activation, sizes and w_transposed (backward: 0
+ * dz_linear, 1 dz_linear_backward); may be 0.                                     */
+int dz_linear_workspace(const dz_linear_args_t* args, int backward, int64_t* bytes);
+int dz_linear(const dz_linear_args_t* args, dz_stream_t stream);
+int dz_linear_backward(const dz_linear_args_t* args, dz_stream_t stream);
 
 /* The clipped policy loss with a KL term and an entropy bonus, and its gradient
  * (csrc/dz_policy_loss.hip).  Row i: log-softmax of logits[i], rho = exp(logp - old_logp),

@@ -100,7 +100,7 @@ def act(z, name):
   if name == 'none':
     return z
   if name == 'relu':
-    return np.where(z > 0, z, 0 * z)
+    return np.where(z < 0, 0.0, z)
   if name == 'gelu':
     return 0.5 * z * (1 + erf(z / np.sqrt(2)))
   return z / (1 + np.exp(-z))
