@@ -28,4 +28,12 @@ __device__ __forceinline__ void dz_glds16(const float* src, unsigned lds_byte) {
                  : "=&s"(keep) : "v"(src), "s"(lds_byte) : "memory");
 }
 
+// The same from a scalar base and a 32-bit unsigned byte offset per lane.
+__device__ __forceinline__ void dz_glds16_base(const void* base, unsigned offset, unsigned lds_byte) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
+               "global_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(offset), "s"(base), "s"(lds_byte) : "memory");
+}
+
 }  // namespace

@@ -6,7 +6,6 @@
 
 struct DzGemmPlan {
   int tile;            // index of the tile sizes
-  bool dma;
   int splits, k_split;
   int64_t slab_bytes;  // 0 without splits
 };
@@ -15,11 +14,12 @@ struct DzGemmPlan {
 struct DzLinearLaunch {
   int (*gemm)(const DzGemmArgs&, const DzGemmPlan&, bool a_kc, bool b_kc, hipStream_t);
   int (*dact)(const DzDactArgs&, int chunks, hipStream_t);
+  int (*pack)(const DzPackArgs&, hipStream_t);   // two.src may be NULL
   int (*db)(const float* sums, int chunks, int n, void* db, int db_f32, hipStream_t);
 };
 const DzLinearLaunch* dz_linear_launch_f32();
 const DzLinearLaunch* dz_linear_launch_bf16();
 const DzLinearLaunch* dz_linear_launch_f16();
 
-constexpr DzGemmShape kGemmTiles[] = {{64, 64, 2, 2}, {128, 128, 2, 2}, {256, 256, 2, 4}};
+constexpr DzGemmShape kGemmTiles[] = {{16, 128, 1, 4}, {64, 64, 2, 2}, {128, 128, 2, 2}, {256, 256, 4, 2}};
 constexpr int kGemmTileCount = sizeof(kGemmTiles) / sizeof(kGemmTiles[0]);

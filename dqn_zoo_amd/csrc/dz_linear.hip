@@ -6,6 +6,7 @@
 namespace {
 
 constexpr int kCus = 256;
+constexpr int64_t kMaxPitchBytes = 1 << 24;   // 256 rows of it in a 32-bit offset
 
 const DzLinearLaunch* launches(int dtype) {
   return dtype == DZ_F32 ? dz_linear_launch_f32() : dtype == DZ_BF16 ? dz_linear_launch_bf16()
@@ -14,38 +15,44 @@ const DzLinearLaunch* launches(int dtype) {
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-// Rows at multiples of 16 bytes, and whole 16-byte units of the adjacent index.
-bool unit_aligned(const void* x, int64_t ld, int64_t adjacent, int64_t elem) {
-  const int64_t ve = 16 / elem;
-  return ((uintptr_t)x & 15) == 0 && ld % ve == 0 && adjacent % ve == 0;
-}
+// A matrix in memory: `rows` rows of `cols` adjacent elements, `ld` elements apart.
+struct Matrix { const void* at; int64_t ld, rows, cols; };
 
-// Tile and number of splits: the least estimated time.  A workgroup's stage costs its matrix
-// instructions or its share of the memory system, whichever is more; workgroups run in rounds of
-// the chip; splits add the slabs' way out and back.
-DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool dma) {
+// Whether the main loop can read it where it lies: rows of whole 16-byte units.
+bool readable(const Matrix& x, int64_t elem) {
+  const int64_t ve = 16 / elem;
+  return x.at && ((uintptr_t)x.at & 15) == 0 && x.ld % ve == 0 && x.cols % ve == 0 && x.ld * elem <= kMaxPitchBytes;
+}
+int64_t packed_ld(const Matrix& x, int64_t elem) { return round_up(x.cols, 16 / elem); }
+int64_t packed_bytes(const Matrix& x, int64_t elem) { return round_up(x.rows * packed_ld(x, elem) * elem, 256); }
+
+// Measured on this card (us; sweeps of tiles and splits over 20 shapes): what a stage of a workgroup
+// takes when its CU has nothing else (`alone`, of one workgroup on the chip, up to `full` of 256),
+// and what each of many costs a busy CU.
+struct TileCost { double alone, full, busy; int per_cu; };
+constexpr TileCost kCost16[] = {{0.42, 0.45, 0.20, 4}, {0.45, 0.46, 0.185, 4}, {0.61, 0.95, 0.53, 2}, {1.10, 1.90, 1.90, 1}};
+constexpr TileCost kCost32[] = {{0.55, 0.60, 0.30, 4}, {0.61, 0.62, 0.455, 4}, {2.00, 2.00, 1.85, 2}, {7.20, 7.40, 7.40, 1}};
+
+// Tile and number of splits: the least estimated time.  A split costs its slab's way out and back
+// and a second launch.
+DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool a_kc) {
   DzGemmPlan best{};
-  best.dma = dma;
   double best_us = 1e30;
   const int bk = (int)(128 / elem);
   const int64_t stages = (k + bk - 1) / bk;
-  for (int t = 0; t < (dma ? kGemmTileCount : 2); ++t) {   // (256 x 256 staged through registers would spill)
+  for (int t = a_kc ? 0 : 1; t < kGemmTileCount; ++t) {
     const DzGemmShape g = kGemmTiles[t];
+    const TileCost c = elem == 2 ? kCost16[t] : kCost32[t];
     const int64_t tiles = ((m + g.bm - 1) / g.bm) * ((n + g.bn - 1) / g.bn);
-    const int per_cu = t == 0 ? 4 : t == 1 ? 2 : 1;
     for (int s = 1; s <= kMaxSplits; s *= 2) {
       if (s > 1 && (stages / s < 2 || tiles * s > 4 * kCus)) break;
-      const int64_t depth = (stages + s - 1) / s;
-      // us of one stage of one workgroup alone on its CU: products at ~60 % of the CU's rate
-      const double rate = elem == 2 ? 5.5e6 : 0.5e6;   // flop / us of a CU
-      const double busy = 2.0 * g.bm * g.bn * bk / rate;
-      const int64_t on_chip = tiles * s < (int64_t)kCus * per_cu ? tiles * s : (int64_t)kCus * per_cu;
-      const double rounds = (double)((tiles * s + (int64_t)kCus * per_cu - 1) / ((int64_t)kCus * per_cu));
-      const double sharing = on_chip > kCus ? (double)on_chip / kCus : 1.0;
-      const double latency = 0.5;                      // us a stage takes at least
-      const double stage_us = busy * sharing > latency ? busy * sharing : latency;
-      double us = 2.0 + rounds * depth * stage_us;
-      if (s > 1) us += 3.0 + 2.0 * s * (double)m * n * 4 / 4e6;
+      const int64_t depth = (stages + s - 1) / s, groups = tiles * s;
+      const int64_t per_cu = (groups + kCus - 1) / kCus, rounds = (per_cu + c.per_cu - 1) / c.per_cu;
+      const double load = groups < kCus ? (double)groups / kCus : 1.0;
+      const double one = c.alone + (c.full - c.alone) * load;
+      const double stage = rounds * one > per_cu * c.busy ? rounds * one : per_cu * c.busy;
+      double us = 3.5 + depth * stage;
+      if (s > 1) us += 3.0 + 0.25 * s + 2.0 * s * (double)m * n * 4 / 3e6;
       if (us < best_us) {
         best_us = us;
         best.tile = t;
@@ -59,11 +66,6 @@ DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool dma) {
   return best;
 }
 
-int64_t slab_bytes(int64_t m, int64_t n, int64_t k, int64_t elem) {   // whichever way it will be staged
-  const int64_t a = plan_gemm(m, n, k, elem, true).slab_bytes, b = plan_gemm(m, n, k, elem, false).slab_bytes;
-  return a > b ? a : b;
-}
-
 void use_plan(DzGemmArgs& g, const DzGemmPlan& plan, void* slabs) {
   g.splits = plan.splits;
   g.k_split = plan.k_split;
@@ -72,48 +74,80 @@ void use_plan(DzGemmArgs& g, const DzGemmPlan& plan, void* slabs) {
   g.slab_stride = g.m * g.slab_ld;
 }
 
-// rows of one chunk of the column sums: enough workgroups to fill the chip
-int dact_rows(int64_t m, int64_t n) {
-  const int64_t cols = (n + 255) / 256;
-  int64_t chunks = 4 * kCus / cols;
-  if (chunks < 1) chunks = 1;
-  int64_t rows = round_up((m + chunks - 1) / chunks, 4);
-  return (int)(rows < 32 ? 32 : rows);
+Matrix x_of(const dz_linear_args_t* a) { return {a->x, a->ldx, a->m, a->k}; }
+Matrix w_of(const dz_linear_args_t* a) {
+  return a->w_transposed ? Matrix{a->w, a->ldw, a->n, a->k} : Matrix{a->w, a->ldw, a->k, a->n};
 }
 
-struct BackwardPlan {
- bool dz;                       // dz is formed in the workspace
-  int64_t ld_dz;
-  int rows, chunks;
-  int64_t dz_at, sums_at, slabs_at, bytes;
+// What a call keeps in its workspace, from its start.  (`a` may have no pointers yet: an operand
+// without an address is taken to need its copy.)
+struct Layout {
+  bool pack_x, pack_w, form_dz;
+  DzGemmPlan fwd, dx, dw;
+  int64_t x_at, w_at, dz_at, sums_at, slabs_at, bytes;
+  int rows, chunks;          // of the column sums
 };
 
-BackwardPlan plan_backward(const dz_linear_args_t* a) {
-  BackwardPlan b{};
+Layout plan_forward(const dz_linear_args_t* a) {
+  Layout l{};
   const int64_t elem = dz_elem_bytes(a->dtype);
-  b.dz = a->activation != DZ_ACT_NONE;
-  b.ld_dz = round_up(a->n, 16 / elem);
-  b.rows = dact_rows(a->m, a->n);
-  b.chunks = (int)((a->m + b.rows - 1) / b.rows);
-  int64_t at = 0;
-  b.dz_at = at;
-  if (b.dz) at += round_up(a->m * b.ld_dz * elem, 256);
-  b.sums_at = at;
-  if (b.chunks > 1) at += round_up((int64_t)b.chunks * a->n * 4, 256);
-  b.slabs_at = at;
-  const int64_t dx = slab_bytes(a->m, a->k, a->n, elem);
-  const int64_t dw = a->w_transposed ? slab_bytes(a->n, a->k, a->m, elem) : slab_bytes(a->k, a->n, a->m, elem);
-  b.bytes = at + (dx > dw ? dx : dw);
-  return b;
+  l.pack_x = !readable(x_of(a), elem);
+  l.pack_w = !readable(w_of(a), elem);
+  l.fwd = plan_gemm(a->m, a->n, a->k, elem, true);
+  if (l.pack_x) { l.x_at = l.bytes; l.bytes += packed_bytes(x_of(a), elem); }
+  if (l.pack_w) { l.w_at = l.bytes; l.bytes += packed_bytes(w_of(a), elem); }
+  l.slabs_at = l.bytes;
+  l.bytes += l.fwd.slab_bytes;
+  return l;
+}
+
+Layout plan_backward(const dz_linear_args_t* a) {
+  Layout l{};
+  const int64_t elem = dz_elem_bytes(a->dtype);
+  const bool sizes_only = !a->dy, dx = sizes_only || a->dx, dw = sizes_only || a->dw, db = sizes_only || a->db;
+  const Matrix dy{a->dy, a->lddy, a->m, a->n};
+  l.form_dz = (dx || dw) && (a->activation != DZ_ACT_NONE || !readable(dy, elem));
+  l.pack_x = dw && !readable(x_of(a), elem);
+  l.pack_w = dx && !readable(w_of(a), elem);
+  if (dx) l.dx = plan_gemm(a->m, a->k, a->n, elem, true);
+  if (dw) l.dw = a->w_transposed ? plan_gemm(a->n, a->k, a->m, elem, false) : plan_gemm(a->k, a->n, a->m, elem, false);
+  // rows of one chunk of the column sums: four workgroups per CU, if the rows allow
+  const int64_t cols = (a->n + 64 * (16 / elem) - 1) / (64 * (16 / elem));
+  const int64_t wanted = 4 * kCus / cols < 1 ? 1 : 4 * kCus / cols;
+  const int64_t rows = round_up((a->m + wanted - 1) / wanted, 8);
+  l.rows = (int)(rows < 32 ? 32 : rows);
+  l.chunks = (int)((a->m + l.rows - 1) / l.rows);
+  if (l.pack_x) { l.x_at = l.bytes; l.bytes += packed_bytes(x_of(a), elem); }
+  if (l.pack_w) { l.w_at = l.bytes; l.bytes += packed_bytes(w_of(a), elem); }
+  if (l.form_dz) { l.dz_at = l.bytes; l.bytes += packed_bytes(dy, elem); }
+  if (db && l.chunks > 1) { l.sums_at = l.bytes; l.bytes += round_up((int64_t)l.chunks * a->n * 4, 256); }
+  l.slabs_at = l.bytes;
+  l.bytes += l.dx.slab_bytes > l.dw.slab_bytes ? l.dx.slab_bytes : l.dw.slab_bytes;
+  return l;
+}
+
+// x and w as the main loop reads them, copied first where they have to be
+int operands(const dz_linear_args_t* a, const Layout& l, Matrix& x, Matrix& w, hipStream_t s) {
+  const int64_t elem = dz_elem_bytes(a->dtype);
+  char* ws = (char*)a->ws;
+  x = x_of(a);
+  w = w_of(a);
+  DzPackArgs p{};
+  auto copy = [&](Matrix& q, int64_t at) {
+    DzPackArgs::One& one = p.one.src ? p.two : p.one;
+    one = {q.at, q.ld, q.rows, (int)q.cols, ws + at, packed_ld(q, elem)};
+    q.at = one.dst;
+    q.ld = one.ldd;
+  };
+  if (l.pack_x) copy(x, l.x_at);
+  if (l.pack_w) copy(w, l.w_at);
+  return p.one.src ? launches(a->dtype)->pack(p, s) : DZ_OK;
 }
 
 bool sizes_ok(const dz_linear_args_t* a) {
-  const int64_t most = (1ll << 31) - 1024;
-  return a && dz_is_dtype(a->dtype) && a->activation >= DZ_ACT_NONE && a->activation <= DZ_ACT_SILU &&
-         a->m > 0 && a->k > 0 && a->n > 0 && a->m < most && a->k < most && a->n < most;
-}
-bool strides_ok(const dz_linear_args_t* a) {
-  return a->x && a->w && a->ldx >= a->k && a->ldw >= (a->w_transposed ? a->k : a->n);
+  if (!a || !dz_is_dtype(a->dtype) || a->activation < DZ_ACT_NONE || a->activation > DZ_ACT_SILU) return false;
+  const int64_t wide = kMaxPitchBytes / dz_elem_bytes(a->dtype);
+  return a->m > 0 && a->k > 0 && a->n > 0 && a->m < (1ll << 31) - 1024 && a->k <= wide && a->n <= wide;
 }
 bool workspace_ok(const dz_linear_args_t* a, int64_t need) {
   return need == 0 || (a->ws && a->ws_bytes >= need && ((uintptr_t)a->ws & 15) == 0);
@@ -123,30 +157,32 @@ bool workspace_ok(const dz_linear_args_t* a, int64_t need) {
 
 extern "C" int dz_linear_workspace(const dz_linear_args_t* a, int backward, int64_t* bytes) {
   DZ_REQUIRE(bytes && sizes_ok(a));
-  *bytes = backward ? plan_backward(a).bytes : slab_bytes(a->m, a->n, a->k, dz_elem_bytes(a->dtype));
+  *bytes = backward ? plan_backward(a).bytes : plan_forward(a).bytes;
   return DZ_OK;
 }
 
 extern "C" int dz_linear(const dz_linear_args_t* a, dz_stream_t stream) {
-  DZ_REQUIRE(sizes_ok(a) && strides_ok(a) && a->y && a->ldy >= a->n);
+  DZ_REQUIRE(sizes_ok(a) && a->x && a->w && a->ldx >= a->k && a->ldw >= (a->w_transposed ? a->k : a->n));
+  DZ_REQUIRE(a->y && a->ldy >= a->n);
   DZ_REQUIRE(!a->residual || a->ldr >= a->n);
   DZ_REQUIRE(!a->preact || a->ldz >= a->n);
-  const int64_t elem = dz_elem_bytes(a->dtype);
-  const DzGemmPlan plan = plan_gemm(
-      a->m, a->n, a->k, elem,
-      unit_aligned(a->x, a->ldx, a->k, elem) && unit_aligned(a->w, a->ldw, a->w_transposed ? a->k : a->n, elem));
-  DZ_REQUIRE(workspace_ok(a, slab_bytes(a->m, a->n, a->k, elem)));
+  const Layout l = plan_forward(a);
+  DZ_REQUIRE(workspace_ok(a, l.bytes));
+  const hipStream_t s = dz_s(stream);
+  Matrix x, w;
+  const int rc = operands(a, l, x, w, s);
+  if (rc != DZ_OK) return rc;
   DzGemmArgs g{};
-  g.a = a->x; g.lda = a->ldx;
-  g.b = a->w; g.ldb = a->ldw;
+  g.a = x.at; g.lda = x.ld;
+  g.b = w.at; g.ldb = w.ld;
   g.m = (int)a->m; g.n = (int)a->n; g.k = (int)a->k;
   g.bias = a->bias; g.bias_f32 = a->bias_f32;
   g.residual = a->residual; g.ldr = a->ldr;
   g.y = a->y; g.ldy = a->ldy;
   g.preact = a->preact; g.ldz = a->ldz;
   g.activation = a->activation;
-  use_plan(g, plan, a->ws);
-  return launches(a->dtype)->gemm(g, plan, true, a->w_transposed != 0, dz_s(stream));
+  use_plan(g, l.fwd, (char*)a->ws + l.slabs_at);
+  return launches(a->dtype)->gemm(g, l.fwd, true, a->w_transposed != 0, s);
 }
 
 extern "C" int dz_linear_backward(const dz_linear_args_t* a, dz_stream_t stream) {
@@ -154,59 +190,52 @@ extern "C" int dz_linear_backward(const dz_linear_args_t* a, dz_stream_t stream)
   DZ_REQUIRE(!a->dx || (a->w && a->ldw >= (a->w_transposed ? a->k : a->n) && a->lddx >= a->k));
   DZ_REQUIRE(!a->dw || (a->x && a->ldx >= a->k && a->lddw >= (a->w_transposed ? a->k : a->n)));
   DZ_REQUIRE(a->activation == DZ_ACT_NONE || (a->preact && a->ldz >= a->n));
-  const BackwardPlan b = plan_backward(a);
-  DZ_REQUIRE(workspace_ok(a, b.bytes));
+  const Layout l = plan_backward(a);
+  DZ_REQUIRE(workspace_ok(a, l.bytes));
   const hipStream_t s = dz_s(stream);
+  const DzLinearLaunch* launch = launches(a->dtype);
   const int64_t elem = dz_elem_bytes(a->dtype);
-  const DzLinearLaunch* l = launches(a->dtype);
   char* ws = (char*)a->ws;
-  const void* dz = a->dy;
-  int64_t lddz = a->lddy;
-  if (b.dz || a->db) {
+  Matrix dz{a->dy, a->lddy, a->m, a->n}, x, w;
+  int rc = DZ_OK;
+  if (l.form_dz || a->db) {
     DzDactArgs d{};
     d.dy = a->dy; d.ldy = a->lddy;
-    if (b.dz) {
-      d.z = a->preact; d.ldz = a->ldz;
-      if (a->dx || a->dw) {
-        d.dz = ws + b.dz_at; d.lddz = b.ld_dz;
-        dz = d.dz; lddz = b.ld_dz;
-      }
+    if (a->activation != DZ_ACT_NONE) { d.z = a->preact; d.ldz = a->ldz; }
+    if (l.form_dz) {
+      d.dz = ws + l.dz_at; d.lddz = packed_ld(dz, elem);
+      dz.at = d.dz; dz.ld = d.lddz;
     }
-    d.m = (int)a->m; d.n = (int)a->n; d.rows = b.rows; d.activation = a->activation;
+    d.m = (int)a->m; d.n = (int)a->n; d.rows = l.rows; d.activation = a->activation;
     if (a->db) {
-      if (b.chunks > 1) d.sums = (float*)(ws + b.sums_at);
+      if (l.chunks > 1) d.sums = (float*)(ws + l.sums_at);
       else { d.db = a->db; d.db_f32 = a->grads_f32; }
     }
-    int rc = l->dact(d, b.chunks, s);
-    if (rc != DZ_OK) return rc;
-    if (d.sums) rc = l->db(d.sums, b.chunks, d.n, a->db, a->grads_f32, s);
+    rc = launch->dact(d, l.chunks, s);
+    if (rc == DZ_OK && d.sums) rc = launch->db(d.sums, l.chunks, d.n, a->db, a->grads_f32, s);
     if (rc != DZ_OK) return rc;
   }
+  rc = operands(a, l, x, w, s);
+  if (rc != DZ_OK) return rc;
   if (a->dx) {   // dx[m][k] = dz[m][n] w[k][n]^T
-    const DzGemmPlan plan = plan_gemm(
-        a->m, a->k, a->n, elem,
-        unit_aligned(dz, lddz, a->n, elem) && unit_aligned(a->w, a->ldw, a->w_transposed ? a->k : a->n, elem));
     DzGemmArgs g{};
-    g.a = dz; g.lda = lddz;
-    g.b = a->w; g.ldb = a->ldw;
+    g.a = dz.at; g.lda = dz.ld;
+    g.b = w.at; g.ldb = w.ld;
     g.m = (int)a->m; g.n = (int)a->k; g.k = (int)a->n;
     g.y = a->dx; g.ldy = a->lddx;
-    use_plan(g, plan, ws + b.slabs_at);
-    const int rc = l->gemm(g, plan, true, a->w_transposed == 0, s);
+    use_plan(g, l.dx, ws + l.slabs_at);
+    rc = launch->gemm(g, l.dx, true, a->w_transposed == 0, s);
     if (rc != DZ_OK) return rc;
   }
   if (a->dw) {   // dw[k][n] = x[m][k]^T dz[m][n], or its transpose in a transposed weight's layout
     const bool t = a->w_transposed != 0;
-    const DzGemmPlan plan = plan_gemm(t ? a->n : a->k, t ? a->k : a->n, a->m, elem,
-                                      unit_aligned(dz, lddz, a->n, elem) && unit_aligned(a->x, a->ldx, a->k, elem));
     DzGemmArgs g{};
-    g.a = t ? dz : a->x; g.lda = t ? lddz : a->ldx;
-    g.b = t ? a->x : dz; g.ldb = t ? a->ldx : lddz;
+    g.a = t ? dz.at : x.at; g.lda = t ? dz.ld : x.ld;
+    g.b = t ? x.at : dz.at; g.ldb = t ? x.ld : dz.ld;
     g.m = (int)(t ? a->n : a->k); g.n = (int)(t ? a->k : a->n); g.k = (int)a->m;
     g.y = a->dw; g.ldy = a->lddw; g.y_f32 = a->grads_f32;
-    use_plan(g, plan, ws + b.slabs_at);
-    const int rc = l->gemm(g, plan, false, false, s);
-    if (rc != DZ_OK) return rc;
+    use_plan(g, l.dw, ws + l.slabs_at);
+    rc = launch->gemm(g, l.dw, false, false, s);
   }
-  return DZ_OK;
+  return rc;
 }

@@ -14,9 +14,10 @@
 // 16 block, float32 ones by ds_read_b32; the 32-byte (64-byte) columns of a row are permuted by k & 7
 // ((k >> 2) & 3), which puts the rows of one read in different banks.
 //
-// Two ways into LDS: 16-byte LDS-DMA (rows that begin at multiples of 16 bytes and hold whole units;
-// what is past an edge reads a clamped address and, along k, is zeroed in LDS before the stage is
-// used), or through registers with a check per unit (everything else).
+// Both operands come by 16-byte LDS-DMA: their rows begin at multiples of 16 bytes and hold whole
+// 16-byte units (operands that do not are copied into such rows first, linear_pack_kernel, zeros
+// behind their ends).  What is past an edge along the output index is read from a clamped place and
+// not stored; what is past it along k is zeroed in LDS.
 //
 // MFMA 16 x 16 with the operands exchanged (rows of the instruction are columns of D): a lane ends
 // with four adjacent columns of one row, so that bias, residual and outputs are vector accesses.
@@ -43,6 +44,13 @@ struct DzGemmArgs {
   float* slabs; int64_t slab_ld, slab_stride;
 };
 
+struct DzPackArgs {
+  struct One { const void* src; int64_t ld; int64_t rows; int cols; void* dst; int64_t ldd; };
+  One one, two;
+};
+
+// dz = dy act'(z) (or dy) and its column sums over `rows` rows of one workgroup: 64 threads hold 16
+// bytes of columns each, 4 rows at a time.
 struct DzDactArgs {
   const void* dy; int64_t ldy;
   const void* z; int64_t ldz;
@@ -189,60 +197,58 @@ struct Operand {
   }
 };
 
-// The stages of one operand as this thread's units, through registers or by LDS-DMA.
+// The stages of one operand by LDS-DMA: a scalar base that moves by a stage, and one constant 32-bit
+// offset per unit of this thread (no vector arithmetic in the main loop).
 template <typename T, bool KC, int EXT, int THREADS>
 struct Stager {
   using O = Operand<T, KC, EXT>;
-  static constexpr int PER = O::UNITS / THREADS;
-  static_assert(O::UNITS % THREADS == 0, "whole units per thread");
-  DzPack<T, O::VE> r[PER];
+  static constexpr int PIECES = O::UNITS / 64;                            // DMA instructions of a stage
+  static constexpr int PER = (PIECES + THREADS / 64 - 1) / (THREADS / 64);  // of a wave
+  const char* base;
+  int64_t stage_bytes, k_bytes;   // one stage along k; one k
+  unsigned off[PER];
 
-  __device__ static int unit(int n) {   // unit n of this thread: a wave's units are adjacent
-    return ((threadIdx.x >> 6) * PER + n) * 64 + (threadIdx.x & 63);
-  }
-  // units that are whole inside [0, ext) x [0, k_end) are one load; the others go element by element
-  __device__ void load(const T* x, int64_t ld, int i0, int ext, int k0, int k_end) {
+  __device__ static int unit(int n, int wave, int lane) { return (wave * PER + n) * 64 + lane; }
+  // (a short operand has fewer pieces than there are waves)
+  __device__ static bool has(int n, int wave) { return PIECES % (THREADS / 64) == 0 || wave * PER + n < PIECES; }
+  // what lies past the edge along the output index is read from a clamped place: its products are
+  // not stored
+  __device__ void init(const T* x, int64_t ld, int i0, int ext, int k0, int wave, int lane) {
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
       int i, k;
-      O::place(unit(n), i, k);
-      i += i0;
-      k += k0;
-      const bool whole = KC ? (i < ext && k + O::VE <= k_end) : (i + O::VE <= ext && k < k_end);
-      if (whole) {
-        r[n] = dz_load<T, O::VE>(KC ? x + i * ld + k : x + k * ld + i);
-      } else {
+      O::place(unit(n, wave, lane), i, k);
+      i = min(i + i0, KC ? ext - 1 : (ext - 1) / O::VE * O::VE) - i0;
+      off[n] = (unsigned)((KC ? i * ld + k : k * ld + i) * (int64_t)sizeof(T));
+    }
+    base = (const char*)(KC ? x + i0 * ld + k0 : x + k0 * ld + i0);
+    k_bytes = (KC ? 1 : ld) * (int64_t)sizeof(T);
+    stage_bytes = O::BK * k_bytes;
+  }
+  __device__ void issue(unsigned lds_byte, int wave) {
 #pragma unroll
-        for (int e = 0; e < O::VE; ++e) {
-          const bool in = KC ? (i < ext && k + e < k_end) : (i + e < ext && k < k_end);
-          r[n].v[e] = in ? (KC ? x[i * ld + k + e] : x[k * ld + i + e]) : (T)0.0f;
-        }
-      }
+    for (int n = 0; n < PER; ++n)
+      if (has(n, wave)) dz_glds16_base(base, off[n], lds_byte + (wave * PER + n) * 1024u);
+    base += stage_bytes;
+  }
+  // a stage that is only `rem` deep, `stages` whole ones from here: what lies past it along k is
+  // read from its first k, and zeroed in LDS, by the lanes that asked for it, once it is there
+  __device__ void issue_tail(unsigned lds_byte, int wave, int lane, int rem, int stages) const {
+    const char* tail = base + stages * stage_bytes;
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      int i, k;
+      O::place(unit(n, wave, lane), i, k);
+      const unsigned o = k < rem ? off[n] : off[n] - (unsigned)(k * k_bytes);
+      if (has(n, wave)) dz_glds16_base(tail, o, lds_byte + (wave * PER + n) * 1024u);
     }
   }
-  __device__ void write(char* lds) const {
-#pragma unroll
-    for (int n = 0; n < PER; ++n) *(DzPack<T, O::VE>*)__builtin_assume_aligned(lds + unit(n) * 16, 16) = r[n];
-  }
-  __device__ static void dma(const T* x, int64_t ld, int i0, int ext, int k0, int k_end, unsigned lds_byte) {
-    const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __device__ static void zero_tail(char* lds, int wave, int lane, int rem) {
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
       int i, k;
-      O::place(unit(n), i, k);
-      i = min(i + i0, KC ? ext - 1 : ext - O::VE);
-      k = min(k + k0, KC ? k_end - O::VE : k_end - 1);
-      const T* src = KC ? x + i * ld + k : x + k * ld + i;
-      dz_glds16<0>((const float*)src, lds_byte + (wave * PER + n) * 1024u);
-    }
-  }
-  // the DMA has clamped what is past k_end: zeros in its place, by the lanes that asked for it
-  __device__ static void zero_tail(char* lds, int k0, int k_end) {
-#pragma unroll
-    for (int n = 0; n < PER; ++n) {
-      int i, k;
-      O::place(unit(n), i, k);
-      if (k + k0 >= k_end) *(uint4*)(lds + unit(n) * 16) = make_uint4(0, 0, 0, 0);
+      O::place(unit(n, wave, lane), i, k);
+      if (has(n, wave) && k >= rem) *(uint4*)(lds + unit(n, wave, lane) * 16) = make_uint4(0, 0, 0, 0);
     }
   }
 };
@@ -258,7 +264,7 @@ __device__ __forceinline__ void tile_of(int id, int tiles, int tiles_m, int tile
   tn = in / rows;
 }
 
-template <typename T, bool A_KC, bool B_KC, bool DMA, int BM, int BN, int WM, int WN>
+template <typename T, bool A_KC, bool B_KC, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void linear_gemm_kernel(DzGemmArgs p) {
   constexpr int THREADS = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, BK = 128 / sizeof(T);
   constexpr int A_BYTES = BM * 128, STAGE = (BM + BN) * 128;
@@ -277,64 +283,61 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_gemm_kernel(DzGemmArgs p)
   const T* b = (const T*)p.b;
   const unsigned lds0 = (unsigned)(uintptr_t)lds;
 
+  const int rem = (k_end - k0) % BK;   // a stage that is not whole is taken first, out of the main loop
+
   f32x4 acc[FM][FN] = {};
   SA ra;
   SB rb;
-  auto fetch = [&](int t, int buf) {
-    const int k = k0 + t * BK;
-    if constexpr (DMA) {
-      SA::dma(a, p.lda, i0, p.m, k, k_end, lds0 + buf * STAGE);
-      SB::dma(b, p.ldb, j0, p.n, k, k_end, lds0 + buf * STAGE + A_BYTES);
-    } else {
-      ra.load(a, p.lda, i0, p.m, k, k_end);
-      rb.load(b, p.ldb, j0, p.n, k, k_end);
-    }
+  ra.init(a, p.lda, i0, p.m, k0, wave, lane);
+  rb.init(b, p.ldb, j0, p.n, k0, wave, lane);
+  auto fetch = [&](int buf) {
+    ra.issue(lds0 + buf * STAGE, wave);
+    rb.issue(lds0 + buf * STAGE + A_BYTES, wave);
   };
-  auto arrive = [&](int t, int buf) {   // stage t is whole in LDS, for every wave
-    char* s = lds + buf * STAGE;
-    if constexpr (DMA) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      const int k = k0 + t * BK;
-      if (k + BK > k_end) {
-        SA::zero_tail(s, k, k_end);
-        SB::zero_tail(s + A_BYTES, k, k_end);
-      }
-    } else {
-      ra.write(s);
-      rb.write(s + A_BYTES);
-    }
-    __syncthreads();
-  };
-  if (stages > 0) {
-    fetch(0, 0);
-    arrive(0, 0);
+  auto land = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };   // this wave's DMAs are in LDS
+  if (rem) {
+    ra.issue_tail(lds0, wave, lane, rem, stages - 1);
+    rb.issue_tail(lds0 + A_BYTES, wave, lane, rem, stages - 1);
+    land();
+    SA::zero_tail(lds, wave, lane, rem);
+    SB::zero_tail(lds + A_BYTES, wave, lane, rem);
+  } else {
+    fetch(0);
+    land();
   }
-  for (int t = 0; t < stages; ++t) {
-    const int buf = t & 1;
-    if (t + 1 < stages) fetch(t + 1, buf ^ 1);
+  __syncthreads();
+  auto step = [&](int t, int buf) {
+    if (t + 1 < stages) fetch(buf ^ 1);
     const char* sa = lds + buf * STAGE;
     const char* sb = sa + A_BYTES;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       typename MfmaFrag<T>::V fa[FM], fb[FN];
 #pragma unroll
-      for (int f = 0; f < FM; ++f) fa[f] = Operand<T, A_KC, BM>::fragment(sa, wm * FM + f, s, lane);
-#pragma unroll
       for (int f = 0; f < FN; ++f) fb[f] = Operand<T, B_KC, BN>::fragment(sb, wn * FN + f, s, lane);
+#pragma unroll
+      for (int f = 0; f < FM; ++f) fa[f] = Operand<T, A_KC, BM>::fragment(sa, wm * FM + f, s, lane);
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = mfma16(fb[j], fa[i], acc[i][j]);
     }
-    if (t + 1 < stages) arrive(t + 1, buf ^ 1);
+    land();
+    __syncthreads();   // the next stage is there, and nobody reads this one any more
+  };
+  int t = 0;
+  for (; t + 2 <= stages; t += 2) {   // (constant LDS addresses)
+    step(t, 0);
+    step(t + 1, 1);
   }
+  if (t < stages) step(t, 0);
 
   // Through LDS, so that 16 lanes hold 64 adjacent columns of a row: whole lines to memory, and one
   // copy of the epilogue's code for each pass of up to 64 rows.  16-byte unit u of row r lies in
   // place u ^ (r & 15 or 7): the writes (16 rows each) start in different banks.
-  constexpr int TN = BN / WN, UPR = TN / 4, PASS = FM < 4 ? FM : 4;
-  static_assert(WM * WN * PASS * 16 * TN * 4 <= 2 * STAGE, "a pass fits the stage buffers");
-  __syncthreads();   // (every wave has read its last stage)
+  constexpr int TN = BN / WN, UPR = TN / 4, FIT = 2 * STAGE / (WM * WN * 16 * TN * 4);
+  constexpr int PASS = FM <= FIT ? FM : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
+  static_assert(FIT >= 1 && FM % PASS == 0, "whole passes that fit the stage buffers");
   float* mine = (float*)lds + wave * (PASS * 16 * TN);
 #pragma unroll
   for (int h = 0; h < FM / PASS; ++h) {
@@ -364,6 +367,27 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_gemm_kernel(DzGemmArgs p)
   }
 }
 
+// Copies one or two operands into rows of whole 16-byte units, zeros behind their ends: a unit per
+// thread.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_pack_kernel(DzPackArgs p) {
+  constexpr int VE = 16 / sizeof(T);
+  const DzPackArgs::One q = blockIdx.y ? p.two : p.one;
+  const int64_t per_row = q.ldd / VE, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= per_row * q.rows) return;
+  const int64_t row = id / per_row;
+  const int c = (int)(id - row * per_row) * VE;
+  const T* x = (const T*)q.src + row * q.ld + c;
+  DzPack<T, VE> v;
+  if (c + VE <= q.cols) {
+    v = dz_load<T, VE>(x);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v.v[e] = c + e < q.cols ? x[e] : (T)0.0f;
+  }
+  dz_store<T, VE>((T*)q.dst + row * q.ldd + c, v);
+}
+
 // The splits' slabs, added in order, and the epilogue: four columns per thread.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_finish_kernel(DzGemmArgs p) {
@@ -372,71 +396,87 @@ __global__ __launch_bounds__(256) void linear_finish_kernel(DzGemmArgs p) {
   const int64_t row = id / per_row;
   const int c = (int)(id - row * per_row) * 4;
   if (c >= p.n) return;
-  float4 s = *(const float4*)(p.slabs + row * p.slab_ld + c);
-  for (int k = 1; k < p.splits; ++k) {
-    const float4 x = *(const float4*)(p.slabs + k * p.slab_stride + row * p.slab_ld + c);
-    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  const float* at = p.slabs + row * p.slab_ld + c;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < p.splits; k += 8) {   // eight loads in flight; the sums in order
+    float4 x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = *(const float4*)(at + min(k + e, p.splits - 1) * p.slab_stride);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (k + e >= p.splits) break;
+      s.x += x[e].x; s.y += x[e].y; s.z += x[e].z; s.w += x[e].w;
+    }
   }
   const float d[4] = {s.x, s.y, s.z, s.w};
   linear_epilogue<T>(p, row, c, d);
 }
 
-// dz = dy act'(z) (or dy) and its column sums over `rows` rows of one workgroup: 64 threads hold 4
-// columns each, 4 rows at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dact_kernel(DzDactArgs p) {
-  const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4, r = threadIdx.x >> 6;
-  const int count = min(4, p.n - c);
+  constexpr int VE = 16 / sizeof(T);
+  const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * VE, r = threadIdx.x >> 6;
+  const int count = min(VE, p.n - c);
   const int64_t first = (int64_t)blockIdx.y * p.rows, end = min((int64_t)p.m, first + p.rows);
-  float s[4] = {};
-  if (count > 0) {
+  float s[VE] = {};
+  auto row = [&](int64_t i, DzPack<T, VE> d, DzPack<T, VE> z) {
+    float y[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      y[e] = (float)d.v[e];
+      if (p.z) y[e] *= linear_act_slope((float)z.v[e], p.activation);
+      s[e] += y[e];
+    }
+    if (!p.dz) return;
+    T* o = (T*)p.dz + i * p.lddz + c;
+    if (count == VE) {
+      dz_store<T, VE>(o, dz_round<T, VE>(y));
+    } else {
+      // (dz's rows are padded to whole units; what is behind their ends is 0)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) y[e] = e < count ? y[e] : 0.f;
+      dz_store<T, VE>(o, dz_round<T, VE>(y));
+    }
+  };
+  const T* dy = (const T*)p.dy + c;
+  const T* z = (const T*)p.z + c;
+  if (count == VE) {
+    for (int64_t i = first + r; i < end; i += 8) {   // two rows in flight
+      const bool two = i + 4 < end;
+      const int64_t j = two ? i + 4 : i;
+      DzPack<T, VE> z0, z1;
+      const auto d0 = dz_load<T, VE>(dy + i * p.ldy), d1 = dz_load<T, VE>(dy + j * p.ldy);
+      if (p.z) {
+        z0 = dz_load<T, VE>(z + i * p.ldz);
+        z1 = dz_load<T, VE>(z + j * p.ldz);
+      }
+      row(i, d0, z0);
+      if (two) row(j, d1, z1);
+    }
+  } else if (count > 0) {
     for (int64_t i = first + r; i < end; i += 4) {
-      DzPack<T, 4> d, z;
-      const T* dy = (const T*)p.dy + i * p.ldy + c;
-      const T* zi = (const T*)p.z + i * p.ldz + c;
-      if (count == 4) {
-        d = dz_load<T, 4>(dy);
-        if (p.z) z = dz_load<T, 4>(zi);
-      } else {
+      DzPack<T, VE> d0, z0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          d.v[e] = e < count ? dy[e] : (T)0.0f;
-          if (p.z) z.v[e] = e < count ? zi[e] : (T)0.0f;
-        }
+      for (int e = 0; e < VE; ++e) {
+        d0.v[e] = e < count ? dy[i * p.ldy + e] : (T)0.0f;
+        z0.v[e] = p.z && e < count ? z[i * p.ldz + e] : (T)0.0f;
       }
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = (float)d.v[e];
-        if (p.z) y[e] *= linear_act_slope((float)z.v[e], p.activation);
-        s[e] += y[e];
-      }
-      if (p.dz) {
-        T* o = (T*)p.dz + i * p.lddz + c;
-        if (count == 4) {
-          dz_store<T, 4>(o, dz_round<T, 4>(y));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e < count) o[e] = (T)y[e];
-        }
-      }
+      row(i, d0, z0);
     }
   }
   if (!p.sums && !p.db) return;
-  __shared__ float4 red[4][64];
-  red[r][threadIdx.x & 63] = make_float4(s[0], s[1], s[2], s[3]);
+  __shared__ float red[4][VE][64];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) red[r][e][threadIdx.x & 63] = s[e];
   __syncthreads();
   if (r || count <= 0) return;
-  const float4 q0 = red[0][threadIdx.x], q1 = red[1][threadIdx.x], q2 = red[2][threadIdx.x], q3 = red[3][threadIdx.x];
-  const float o[4] = {(q0.x + q1.x) + (q2.x + q3.x), (q0.y + q1.y) + (q2.y + q3.y),
-                      (q0.z + q1.z) + (q2.z + q3.z), (q0.w + q1.w) + (q2.w + q3.w)};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < VE; ++e) {
     if (e >= count) break;
-    if (p.sums) p.sums[(int64_t)blockIdx.y * p.n + c + e] = o[e];
-    else if (p.db_f32) ((float*)p.db)[c + e] = o[e];
-    else ((T*)p.db)[c + e] = (T)o[e];
+    const float o = (red[0][e][threadIdx.x] + red[1][e][threadIdx.x]) + (red[2][e][threadIdx.x] + red[3][e][threadIdx.x]);
+    if (p.sums) p.sums[(int64_t)blockIdx.y * p.n + c + e] = o;
+    else if (p.db_f32) ((float*)p.db)[c + e] = o;
+    else ((T*)p.db)[c + e] = (T)o;
   }
 }
 
@@ -447,7 +487,14 @@ __global__ __launch_bounds__(256) void linear_db_kernel(const float* __restrict_
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= n) return;
   float s = 0.f;
-  for (int i = 0; i < chunks; ++i) s += sums[(int64_t)i * n + c];
+  for (int i = 0; i < chunks; i += 8) {   // eight loads in flight; the sums in order
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = sums[(int64_t)min(i + e, chunks - 1) * n + c];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < chunks) s += x[e];
+  }
   if (db_f32) ((float*)db)[c] = s;
   else ((T*)db)[c] = (T)s;
 }

@@ -5,13 +5,13 @@
 
 namespace {
 
-template <typename T, bool A_KC, bool B_KC, bool DMA, int TILE>
+template <typename T, bool A_KC, bool B_KC, int TILE>
 int launch_gemm_tile(const DzGemmArgs& p, hipStream_t s) {
   constexpr DzGemmShape t = kGemmTiles[TILE];
   constexpr int kLds = 2 * (t.bm + t.bn) * 128;
   const int64_t tiles = (int64_t)((p.m + t.bm - 1) / t.bm) * ((p.n + t.bn - 1) / t.bn);
   if (tiles >= (1ll << 31)) return DZ_ERR_UNSUPPORTED;
-  auto kernel = linear_gemm_kernel<T, A_KC, B_KC, DMA, t.bm, t.bn, t.wm, t.wn>;
+  auto kernel = linear_gemm_kernel<T, A_KC, B_KC, t.bm, t.bn, t.wm, t.wn>;
   if (kLds > 65536)
     DZ_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
   hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)p.splits), dim3(64 * t.wm * t.wn), kLds, s, p);
@@ -21,13 +21,13 @@ int launch_gemm_tile(const DzGemmArgs& p, hipStream_t s) {
 
 template <typename T, bool A_KC, bool B_KC>
 int launch_gemm_kind(const DzGemmArgs& p, const DzGemmPlan& plan, hipStream_t s) {
-  switch (plan.tile * 2 + plan.dma) {
-    case 0: return launch_gemm_tile<T, A_KC, B_KC, false, 0>(p, s);
-    case 1: return launch_gemm_tile<T, A_KC, B_KC, true, 0>(p, s);
-    case 2: return launch_gemm_tile<T, A_KC, B_KC, false, 1>(p, s);
-    case 3: return launch_gemm_tile<T, A_KC, B_KC, true, 1>(p, s);
-    case 4: return launch_gemm_tile<T, A_KC, B_KC, false, 2>(p, s);
-    case 5: return launch_gemm_tile<T, A_KC, B_KC, true, 2>(p, s);
+  switch (plan.tile) {
+    case 0:   // (16 rows: only where the rows of A lie one behind the other)
+      if constexpr (A_KC) return launch_gemm_tile<T, A_KC, B_KC, 0>(p, s);
+      return DZ_ERR_UNSUPPORTED;
+    case 1: return launch_gemm_tile<T, A_KC, B_KC, 1>(p, s);
+    case 2: return launch_gemm_tile<T, A_KC, B_KC, 2>(p, s);
+    case 3: return launch_gemm_tile<T, A_KC, B_KC, 3>(p, s);
     default: return DZ_ERR_UNSUPPORTED;
   }
 }
@@ -49,7 +49,18 @@ int launch_gemm(const DzGemmArgs& p, const DzGemmPlan& plan, bool a_kc, bool b_k
 
 template <typename T>
 int launch_dact(const DzDactArgs& p, int chunks, hipStream_t s) {
-  hipLaunchKernelGGL((linear_dact_kernel<T>), dim3((p.n + 255) / 256, chunks), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((linear_dact_kernel<T>), dim3((p.n + 64 * (16 / (int)sizeof(T)) - 1) / (64 * (16 / (int)sizeof(T))), chunks), dim3(256), 0, s, p);
+  DZ_LAUNCH_CHECK();
+  return DZ_OK;
+}
+
+template <typename T>
+int launch_pack(const DzPackArgs& p, hipStream_t s) {
+  const int64_t one = p.one.rows * (p.one.ldd / (16 / (int64_t)sizeof(T)));
+  const int64_t two = p.two.src ? p.two.rows * (p.two.ldd / (16 / (int64_t)sizeof(T))) : 0;
+  const int64_t blocks = ((one > two ? one : two) + 255) / 256;
+  if (blocks >= (1ll << 31)) return DZ_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((linear_pack_kernel<T>), dim3((unsigned)blocks, p.two.src ? 2 : 1), dim3(256), 0, s, p);
   DZ_LAUNCH_CHECK();
   return DZ_OK;
 }
@@ -63,7 +74,7 @@ int launch_db(const float* sums, int chunks, int n, void* db, int db_f32, hipStr
 
 template <typename T>
 const DzLinearLaunch* linear_launches() {
-  static const DzLinearLaunch l = {launch_gemm<T>, launch_dact<T>, launch_db<T>};
+  static const DzLinearLaunch l = {launch_gemm<T>, launch_dact<T>, launch_pack<T>, launch_db<T>};
   return &l;
 }
 

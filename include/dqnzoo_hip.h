@@ -834,7 +834,7 @@ int dz_adamw_moments(const uint8_t* m, const uint8_t* v, const float* m_scale, c
 #define DZ_ACT_SILU 3
 typedef struct {
   int32_t dtype, activation;
-  int64_t m, k, n;           /* each 1 .. 2^31 - 1025                            */
+  int64_t m, k, n;           /* m < 2^31 - 1024; rows of k and of n elements up to 2^24 bytes */
   const void* x; int64_t ldx;
   const void* w; int64_t ldw;
   int32_t w_transposed;
@@ -853,8 +853,10 @@ typedef struct {
   void* ws; int64_t ws_bytes;  /* dz_linear_workspace; 16-byte aligned, contents arbitrary */
 } dz_linear_args_t;
 
-/* Bytes of workspace for these dtype, activation, sizes and w_transposed (backward: 0
- * dz_linear, 1 dz_linear_backward); may be 0.                                     */
+/* Bytes of workspace for the call that these arguments make (backward: 0 dz_linear, 1
+ * dz_linear_backward); may be 0.  Without pointers (x, w, dy NULL): enough for every call
+ * of these dtype, activation, sizes and w_transposed.  Operands whose rows are not whole
+ * 16-byte units at 16-byte addresses are copied into such rows there.              */
 int dz_linear_workspace(const dz_linear_args_t* args, int backward, int64_t* bytes);
 int dz_linear(const dz_linear_args_t* args, dz_stream_t stream);
 int dz_linear_backward(const dz_linear_args_t* args, dz_stream_t stream);
