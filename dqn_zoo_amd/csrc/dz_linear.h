@@ -5,7 +5,7 @@
 #include "dz_linear_gemm.h"
 
 struct DzGemmPlan {
-  int tile;            // index of the tile sizes
+  int tile;            // index of the tile sizes, or kRowsTile
   int splits, k_split;
   int64_t slab_bytes;  // 0 without splits
 };
@@ -21,5 +21,6 @@ const DzLinearLaunch* dz_linear_launch_f32();
 const DzLinearLaunch* dz_linear_launch_bf16();
 const DzLinearLaunch* dz_linear_launch_f16();
 
-constexpr DzGemmShape kGemmTiles[] = {{16, 128, 1, 4}, {64, 64, 2, 2}, {128, 128, 2, 2}, {256, 256, 4, 2}};
+constexpr DzGemmShape kGemmTiles[] = {{64, 64, 2, 2, 3}, {128, 128, 2, 2, 2}, {256, 256, 2, 4, 2}};
 constexpr int kGemmTileCount = sizeof(kGemmTiles) / sizeof(kGemmTiles[0]);
+constexpr int kRowsTile = -1;   // linear_rows_kernel: up to kRowsM rows

@@ -26,21 +26,33 @@ bool readable(const Matrix& x, int64_t elem) {
 int64_t packed_ld(const Matrix& x, int64_t elem) { return round_up(x.cols, 16 / elem); }
 int64_t packed_bytes(const Matrix& x, int64_t elem) { return round_up(x.rows * packed_ld(x, elem) * elem, 256); }
 
-// Measured on this card (us; sweeps of tiles and splits over 20 shapes): what a stage of a workgroup
+// Measured on this card (us; sweeps of tiles and splits over 30 shapes): what a stage of a workgroup
 // takes when its CU has nothing else (`alone`, of one workgroup on the chip, up to `full` of 256),
 // and what each of many costs a busy CU.
 struct TileCost { double alone, full, busy; int per_cu; };
-constexpr TileCost kCost16[] = {{0.42, 0.45, 0.20, 4}, {0.45, 0.46, 0.185, 4}, {0.61, 0.95, 0.53, 2}, {1.10, 1.90, 1.90, 1}};
-constexpr TileCost kCost32[] = {{0.55, 0.60, 0.30, 4}, {0.61, 0.62, 0.455, 4}, {2.00, 2.00, 1.85, 2}, {7.20, 7.40, 7.40, 1}};
+constexpr TileCost kCost16[] = {{0.22, 0.25, 0.185, 3}, {0.61, 0.95, 0.53, 2}, {1.10, 1.90, 1.90, 1}};
+constexpr TileCost kCost32[] = {{0.58, 0.60, 0.455, 3}, {2.00, 2.00, 1.85, 2}, {7.20, 7.40, 7.40, 1}};
 
-// Tile and number of splits: the least estimated time.  A split costs its slab's way out and back
-// and a second launch.
-DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool a_kc) {
+// Tile and number of splits: the least estimated time, with the operands' bytes at 5.3 TB/s as its
+// floor.  A split costs its slab's way out and back and a second launch.  Up to 16 rows may take the
+// rows' kernel: 1 x 3136 x 512 in 5.2 us against 8.7 (tile 64 x 64, 7 splits), 16 x 8192 x 4096 from
+// a transposed weight in 15.0 against 15.7; its 64-byte pieces of an (in, out) weight's rows come at
+// 2.4 TB/s (16 x 8192 x 4096: 25.8 against 16.8).
+DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool a_kc, bool b_kc) {
   DzGemmPlan best{};
   double best_us = 1e30;
   const int bk = (int)(128 / elem);
   const int64_t stages = (k + bk - 1) / bk;
-  for (int t = a_kc ? 0 : 1; t < kGemmTileCount; ++t) {
+  const double bytes = (double)(m + n) * k * elem;
+  if (a_kc && m <= kRowsM) {
+    const int64_t rounds = ((n + kRowsN - 1) / kRowsN + kCus - 1) / kCus, depth = (stages + kRowsWaves - 1) / kRowsWaves;
+    const double work = rounds * depth * (elem == 2 ? 0.30 : 0.56), flow = bytes / (b_kc || elem == 4 ? 5.3e6 : 2.4e6);
+    best_us = 3.0 + (work > flow ? work : flow) + 0.9 * (rounds - 1);
+    best.tile = kRowsTile;
+    best.splits = 1;
+    best.k_split = (int)(stages * bk);
+  }
+  for (int t = 0; t < kGemmTileCount; ++t) {
     const DzGemmShape g = kGemmTiles[t];
     const TileCost c = elem == 2 ? kCost16[t] : kCost32[t];
     const int64_t tiles = ((m + g.bm - 1) / g.bm) * ((n + g.bn - 1) / g.bn);
@@ -51,8 +63,8 @@ DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool a_kc) {
       const double load = groups < kCus ? (double)groups / kCus : 1.0;
       const double one = c.alone + (c.full - c.alone) * load;
       const double stage = rounds * one > per_cu * c.busy ? rounds * one : per_cu * c.busy;
-      double us = 3.5 + depth * stage;
-      if (s > 1) us += 3.0 + 0.25 * s + 2.0 * s * (double)m * n * 4 / 3e6;
+      double us = 3.5 + (depth * stage > bytes / 5.3e6 ? depth * stage : bytes / 5.3e6);
+      if (s > 1) us += 2.8 + 0.1 * s + 2.0 * s * (double)m * n * 4 / 3e6;
       if (us < best_us) {
         best_us = us;
         best.tile = t;
@@ -62,7 +74,7 @@ DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool a_kc) {
     }
   }
   best.splits = (int)((stages + best.k_split / bk - 1) / (best.k_split / bk));
-  best.slab_bytes = best.splits > 1 ? best.splits * m * round_up(n, 4) * 4 : 0;
+  best.slab_bytes = best.splits > 1 ? best.splits * m * round_up(n, 8) * 4 : 0;
   return best;
 }
 
@@ -70,7 +82,7 @@ void use_plan(DzGemmArgs& g, const DzGemmPlan& plan, void* slabs) {
   g.splits = plan.splits;
   g.k_split = plan.k_split;
   g.slabs = (float*)slabs;
-  g.slab_ld = round_up(g.n, 4);
+  g.slab_ld = round_up(g.n, 8);
   g.slab_stride = g.m * g.slab_ld;
 }
 
@@ -93,7 +105,7 @@ Layout plan_forward(const dz_linear_args_t* a) {
   const int64_t elem = dz_elem_bytes(a->dtype);
   l.pack_x = !readable(x_of(a), elem);
   l.pack_w = !readable(w_of(a), elem);
-  l.fwd = plan_gemm(a->m, a->n, a->k, elem, true);
+  l.fwd = plan_gemm(a->m, a->n, a->k, elem, true, a->w_transposed != 0);
   if (l.pack_x) { l.x_at = l.bytes; l.bytes += packed_bytes(x_of(a), elem); }
   if (l.pack_w) { l.w_at = l.bytes; l.bytes += packed_bytes(w_of(a), elem); }
   l.slabs_at = l.bytes;
@@ -109,8 +121,9 @@ Layout plan_backward(const dz_linear_args_t* a) {
   l.form_dz = (dx || dw) && (a->activation != DZ_ACT_NONE || !readable(dy, elem));
   l.pack_x = dw && !readable(x_of(a), elem);
   l.pack_w = dx && !readable(w_of(a), elem);
-  if (dx) l.dx = plan_gemm(a->m, a->k, a->n, elem, true);
-  if (dw) l.dw = a->w_transposed ? plan_gemm(a->n, a->k, a->m, elem, false) : plan_gemm(a->k, a->n, a->m, elem, false);
+  if (dx) l.dx = plan_gemm(a->m, a->k, a->n, elem, true, a->w_transposed == 0);
+  if (dw) l.dw = a->w_transposed ? plan_gemm(a->n, a->k, a->m, elem, false, false)
+                                       : plan_gemm(a->k, a->n, a->m, elem, false, false);
   // rows of one chunk of the column sums: four workgroups per CU, if the rows allow
   const int64_t cols = (a->n + 64 * (16 / elem) - 1) / (64 * (16 / elem));
   const int64_t wanted = 4 * kCus / cols < 1 ? 1 : 4 * kCus / cols;
@@ -172,6 +185,7 @@ extern "C" int dz_linear(const dz_linear_args_t* a, dz_stream_t stream) {
   Matrix x, w;
   const int rc = operands(a, l, x, w, s);
   if (rc != DZ_OK) return rc;
+  const int64_t elem = dz_elem_bytes(a->dtype);
   DzGemmArgs g{};
   g.a = x.at; g.lda = x.ld;
   g.b = w.at; g.ldb = w.ld;
@@ -181,6 +195,8 @@ extern "C" int dz_linear(const dz_linear_args_t* a, dz_stream_t stream) {
   g.y = a->y; g.ldy = a->ldy;
   g.preact = a->preact; g.ldz = a->ldz;
   g.activation = a->activation;
+  // An output that no cache would hold until it is read: 4 - 5 % on 256 MB, nothing on 64.
+  g.stream = a->m * a->n * elem * (a->preact ? 2 : 1) >= (128ll << 20);
   use_plan(g, l.fwd, (char*)a->ws + l.slabs_at);
   return launches(a->dtype)->gemm(g, l.fwd, true, a->w_transposed != 0, s);
 }

@@ -26,7 +26,7 @@
 #include "dz_elem.h"
 #include "dz_glds.h"
 
-struct DzGemmShape { int bm, bn, wm, wn; };
+struct DzGemmShape { int bm, bn, wm, wn, buffers; };
 
 struct DzGemmArgs {
   const void* a; int64_t lda;
@@ -42,6 +42,7 @@ struct DzGemmArgs {
   void* preact; int64_t ldz;
   int activation;
   float* slabs; int64_t slab_ld, slab_stride;
+  int stream;              // y and preact are stored past the caches
 };
 
 struct DzPackArgs {
@@ -84,70 +85,121 @@ __device__ __forceinline__ f32x4 mfma16(MfmaFrag<float>::V a, MfmaFrag<float>::V
   return c;
 }
 
+// Phi(-|z|) of the standard normal, and exp(-z^2 / 2) with it.  16-bit layers take
+// erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2), t = 1 / (1 + 0.3275911 x), of Abramowitz and Stegun
+// 7.1.26: 1.5e-7 absolute, 2^-13 of a bf16 half step near 1, for one exponential and one reciprocal
+// (with erff and expf the GELU kernels were bound by arithmetic: dz of 8192 x 4096 took 62 us, 46 so).
+template <typename T>
+__device__ __forceinline__ float normal_tail(float z, float& density) {
+  if constexpr (sizeof(T) == 4) {
+    density = expf(-0.5f * z * z);
+    return 0.5f * erfcf(fabsf(z) * 0.70710678118654752f);
+  } else {
+    density = __builtin_amdgcn_exp2f(-0.72134752044448170f * (z * z));   // log2(e) / 2
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
+    float q = __builtin_fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+    q = __builtin_fmaf(t, q, 0.5f * 1.421413741f);
+    q = __builtin_fmaf(t, q, 0.5f * -0.284496736f);
+    q = __builtin_fmaf(t, q, 0.5f * 0.254829592f);
+    return q * t * density;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float logistic(float z) {
+  if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-z));
+  else return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
+}
+
+template <typename T>
 __device__ __forceinline__ float linear_act(float z, int act) {
+  float density;
   switch (act) {
     case DZ_ACT_RELU: return z < 0.f ? 0.f : z;   // (NaN stays)
-    case DZ_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case DZ_ACT_SILU: return z / (1.0f + expf(-z));
+    case DZ_ACT_GELU: return __builtin_fmaf(-fabsf(z), normal_tail<T>(z, density), fmaxf(z, 0.f));   // z Phi(z)
+    case DZ_ACT_SILU: return z * logistic<T>(z);
     default: return z;
   }
 }
+template <typename T>
 __device__ __forceinline__ float linear_act_slope(float z, int act) {
   switch (act) {
     case DZ_ACT_RELU: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
-    case DZ_ACT_GELU:
-      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+    case DZ_ACT_GELU: {
+      float density;
+      const float tail = normal_tail<T>(z, density);
+      return __builtin_fmaf(z * 0.39894228040143268f, density, z < 0.f ? tail : 1.0f - tail);
+    }
     case DZ_ACT_SILU: {
-      const float s = 1.0f / (1.0f + expf(-z));
+      const float s = logistic<T>(z);
       return s * (1.0f + z * (1.0f - s));
     }
     default: return 1.f;
   }
 }
 
-// Four adjacent columns of a finished row.
-template <typename T>
-__device__ __forceinline__ void linear_epilogue(const DzGemmArgs& p, int64_t i, int j, const float (&d)[4]) {
-  const int count = min(4, p.n - j);
-  float z[4], y[4];
-  if (count == 4) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) z[c] = d[c];
-    if (p.bias) {
-      if (p.bias_f32) {
-        const auto b = dz_load<float, 4>((const float*)p.bias + j);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) z[c] += b.v[c];
-      } else {
-        const auto b = dz_load<T, 4>((const T*)p.bias + j);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) z[c] += (float)b.v[c];
-      }
-    }
-    if (p.preact) dz_store<T, 4>((T*)p.preact + i * p.ldz + j, dz_round<T, 4>(z));
-#pragma unroll
-    for (int c = 0; c < 4; ++c) y[c] = linear_act(z[c], p.activation);
-    if (p.residual) {
-      const auto r = dz_load<T, 4>((const T*)p.residual + i * p.ldr + j);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) y[c] += (float)r.v[c];
-    }
-    if (p.y_f32) dz_store<float, 4>((float*)p.y + i * p.ldy + j, dz_round<float, 4>(y));
-    else dz_store<T, 4>((T*)p.y + i * p.ldy + j, dz_round<T, 4>(y));
+// W adjacent columns from column j of a finished row: bias, activation, residual and outputs.  The
+// columns' bias is the same for every row of a thread.
+// (16 bytes past the caches; other widths as usual)
+template <typename T, int W>
+__device__ __forceinline__ void store_past(T* p, const DzPack<T, W>& x) {
+  if constexpr (sizeof(x) == 16) {
+    typedef __attribute__((ext_vector_type(4), aligned(2))) unsigned U;
+    U u;
+    __builtin_memcpy(&u, &x, 16);
+    __builtin_nontemporal_store(u, (U*)p);
   } else {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if (c >= count) break;
-      float zc = d[c];
-      if (p.bias) zc += p.bias_f32 ? ((const float*)p.bias)[j + c] : (float)((const T*)p.bias)[j + c];
-      if (p.preact) ((T*)p.preact)[i * p.ldz + j + c] = (T)zc;
-      float yc = linear_act(zc, p.activation);
-      if (p.residual) yc += (float)((const T*)p.residual)[i * p.ldr + j + c];
-      if (p.y_f32) ((float*)p.y)[i * p.ldy + j + c] = yc;
-      else ((T*)p.y)[i * p.ldy + j + c] = (T)yc;
-    }
+    dz_store<T, W>(p, x);
   }
 }
+
+template <typename T, int W>
+struct Epilogue {
+  float bias[W];
+  int count;   // columns inside the matrix
+
+  __device__ void init(const DzGemmArgs& p, int j) {
+    count = min(W, p.n - j);
+#pragma unroll
+    for (int c = 0; c < W; ++c) {
+      bias[c] = 0.f;
+      if (p.bias && c < count) bias[c] = p.bias_f32 ? ((const float*)p.bias)[j + c] : (float)((const T*)p.bias)[j + c];
+    }
+  }
+  __device__ void row(const DzGemmArgs& p, int64_t i, int j, const float (&d)[W]) const {
+    T* pre = (T*)p.preact + i * p.ldz + j;
+    const T* res = (const T*)p.residual + i * p.ldr + j;
+    float z[W], y[W];
+#pragma unroll
+    for (int c = 0; c < W; ++c) z[c] = d[c] + bias[c];
+    if (count == W) {
+      DzPack<T, W> r;
+      if (p.residual) r = dz_load<T, W>(res);
+      if (p.preact) {
+        if (p.stream) store_past<T, W>(pre, dz_round<T, W>(z));
+        else dz_store<T, W>(pre, dz_round<T, W>(z));
+      }
+#pragma unroll
+      for (int c = 0; c < W; ++c) y[c] = linear_act<T>(z[c], p.activation);
+      if (p.residual) {
+#pragma unroll
+        for (int c = 0; c < W; ++c) y[c] += (float)r.v[c];
+      }
+      if (p.y_f32) dz_store<float, W>((float*)p.y + i * p.ldy + j, dz_round<float, W>(y));
+      else if (p.stream) store_past<T, W>((T*)p.y + i * p.ldy + j, dz_round<T, W>(y));
+      else dz_store<T, W>((T*)p.y + i * p.ldy + j, dz_round<T, W>(y));
+    } else {
+#pragma unroll
+      for (int c = 0; c < W; ++c) {
+        if (c >= count) break;
+        if (p.preact) pre[c] = (T)z[c];
+        float v = linear_act<T>(z[c], p.activation);
+        if (p.residual) v += (float)res[c];
+        if (p.y_f32) ((float*)p.y)[i * p.ldy + j + c] = v;
+        else ((T*)p.y)[i * p.ldy + j + c] = (T)v;
+      }
+    }
+  }
+};
 
 // ---- one operand's stage -------------------------------------------------------
 // EXT: rows of the tile along the output index; unit q of the stage is 16 bytes at LDS byte 16 q.
@@ -166,7 +218,7 @@ struct Operand {
       k = q / UPR;
       const int u = q % UPR;
       if constexpr (sizeof(T) == 2) i = (((u >> 1) ^ (k & (EXT / 16 - 1) & 7)) * 2 + (u & 1)) * VE;
-      else i = (((u >> 2) ^ ((k >> 2) & 3)) * 4 + (u & 3)) * VE;
+      else i = (((u >> 2) ^ ((k >> 2) & (EXT / 16 - 1) & 3)) * 4 + (u & 3)) * VE;
     }
   }
   // 16 consecutive output indices from 16 blk, depth step s of 2
@@ -190,7 +242,7 @@ struct Operand {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int k = 16 * s + 4 * g + q;
-        f[q] = *(const float*)(lds + k * (EXT * 4) + ((blk ^ ((k >> 2) & 3)) * 64) + j * 4);
+        f[q] = *(const float*)(lds + k * (EXT * 4) + ((blk ^ ((k >> 2) & (EXT / 16 - 1) & 3)) * 64) + j * 4);
       }
       return f;
     }
@@ -202,15 +254,13 @@ struct Operand {
 template <typename T, bool KC, int EXT, int THREADS>
 struct Stager {
   using O = Operand<T, KC, EXT>;
-  static constexpr int PIECES = O::UNITS / 64;                            // DMA instructions of a stage
-  static constexpr int PER = (PIECES + THREADS / 64 - 1) / (THREADS / 64);  // of a wave
+  static constexpr int PER = O::UNITS / THREADS;
+  static_assert(O::UNITS % THREADS == 0, "whole units per thread");
   const char* base;
   int64_t stage_bytes, k_bytes;   // one stage along k; one k
   unsigned off[PER];
 
   __device__ static int unit(int n, int wave, int lane) { return (wave * PER + n) * 64 + lane; }
-  // (a short operand has fewer pieces than there are waves)
-  __device__ static bool has(int n, int wave) { return PIECES % (THREADS / 64) == 0 || wave * PER + n < PIECES; }
   // what lies past the edge along the output index is read from a clamped place: its products are
   // not stored
   __device__ void init(const T* x, int64_t ld, int i0, int ext, int k0, int wave, int lane) {
@@ -228,7 +278,7 @@ struct Stager {
   __device__ void issue(unsigned lds_byte, int wave) {
 #pragma unroll
     for (int n = 0; n < PER; ++n)
-      if (has(n, wave)) dz_glds16_base(base, off[n], lds_byte + (wave * PER + n) * 1024u);
+      dz_glds16_base(base, off[n], lds_byte + (wave * PER + n) * 1024u);
     base += stage_bytes;
   }
   // a stage that is only `rem` deep, `stages` whole ones from here: what lies past it along k is
@@ -240,7 +290,7 @@ struct Stager {
       int i, k;
       O::place(unit(n, wave, lane), i, k);
       const unsigned o = k < rem ? off[n] : off[n] - (unsigned)(k * k_bytes);
-      if (has(n, wave)) dz_glds16_base(tail, o, lds_byte + (wave * PER + n) * 1024u);
+      dz_glds16_base(tail, o, lds_byte + (wave * PER + n) * 1024u);
     }
   }
   __device__ static void zero_tail(char* lds, int wave, int lane, int rem) {
@@ -248,7 +298,7 @@ struct Stager {
     for (int n = 0; n < PER; ++n) {
       int i, k;
       O::place(unit(n, wave, lane), i, k);
-      if (has(n, wave) && k >= rem) *(uint4*)(lds + unit(n, wave, lane) * 16) = make_uint4(0, 0, 0, 0);
+      if (k >= rem) *(uint4*)(lds + unit(n, wave, lane) * 16) = make_uint4(0, 0, 0, 0);
     }
   }
 };
@@ -264,7 +314,7 @@ __device__ __forceinline__ void tile_of(int id, int tiles, int tiles_m, int tile
   tn = in / rows;
 }
 
-template <typename T, bool A_KC, bool B_KC, int BM, int BN, int WM, int WN>
+template <typename T, bool A_KC, bool B_KC, int BM, int BN, int WM, int WN, int NBUF>
 __global__ __launch_bounds__(64 * WM * WN) void linear_gemm_kernel(DzGemmArgs p) {
   constexpr int THREADS = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, BK = 128 / sizeof(T);
   constexpr int A_BYTES = BM * 128, STAGE = (BM + BN) * 128;
@@ -294,20 +344,30 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_gemm_kernel(DzGemmArgs p)
     ra.issue(lds0 + buf * STAGE, wave);
     rb.issue(lds0 + buf * STAGE + A_BYTES, wave);
   };
-  auto land = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };   // this wave's DMAs are in LDS
+  // Stage t is used from buffer t % NBUF while the NBUF - 1 behind it are on their way.
+  constexpr int AHEAD = NBUF - 2, OUT = AHEAD * (SA::PER + SB::PER);   // stages, DMAs that may still be out
   if (rem) {
     ra.issue_tail(lds0, wave, lane, rem, stages - 1);
     rb.issue_tail(lds0 + A_BYTES, wave, lane, rem, stages - 1);
-    land();
-    SA::zero_tail(lds, wave, lane, rem);
-    SB::zero_tail(lds + A_BYTES, wave, lane, rem);
   } else {
     fetch(0);
-    land();
+  }
+#pragma unroll
+  for (int n = 1; n <= AHEAD; ++n)
+    if (n < stages) fetch(n);
+  auto land = [&](bool all) {   // this wave's DMAs of the next stage (or all) are in LDS
+    if (all || AHEAD == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OUT) : "memory");
+  };
+  land(stages <= AHEAD);
+  if (rem) {
+    SA::zero_tail(lds, wave, lane, rem);
+    SB::zero_tail(lds + A_BYTES, wave, lane, rem);
   }
   __syncthreads();
   auto step = [&](int t, int buf) {
-    if (t + 1 < stages) fetch(buf ^ 1);
+    const bool more = t + NBUF - 1 < stages;
+    if (more) fetch((buf + NBUF - 1) % NBUF);
     const char* sa = lds + buf * STAGE;
     const char* sb = sa + A_BYTES;
 #pragma unroll
@@ -322,94 +382,211 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_gemm_kernel(DzGemmArgs p)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = mfma16(fb[j], fa[i], acc[i][j]);
     }
-    land();
+    land(!more);
     __syncthreads();   // the next stage is there, and nobody reads this one any more
   };
-  int t = 0;
-  for (; t + 2 <= stages; t += 2) {   // (constant LDS addresses)
-    step(t, 0);
-    step(t + 1, 1);
+  if constexpr (!A_KC) {
+    // One copy of the step: the transposing reads take an address per column block and buffer, and
+    // two copies of it spill (256 x 256, 4096 x 4096 x 8192: 228 -> 213 us).
+    int buf = 0;
+#pragma unroll 1
+    for (int t = 0; t < stages; ++t) {
+      step(t, buf);
+      buf = buf == NBUF - 1 ? 0 : buf + 1;
+    }
+  } else {
+    int t = 0;
+    for (; t + NBUF <= stages; t += NBUF) {   // (constant LDS addresses)
+#pragma unroll
+      for (int n = 0; n < NBUF; ++n) step(t + n, n);
+    }
+#pragma unroll
+    for (int n = 0; n < NBUF - 1; ++n)
+      if (t + n < stages) step(t + n, n);
   }
-  if (t < stages) step(t, 0);
 
-  // Through LDS, so that 16 lanes hold 64 adjacent columns of a row: whole lines to memory, and one
-  // copy of the epilogue's code for each pass of up to 64 rows.  16-byte unit u of row r lies in
-  // place u ^ (r & 15 or 7): the writes (16 rows each) start in different banks.
-  constexpr int TN = BN / WN, UPR = TN / 4, FIT = 2 * STAGE / (WM * WN * 16 * TN * 4);
+  // Through LDS, so that a lane holds eight adjacent columns of a row and neighbours make whole lines,
+  // with one copy of the epilogue's code for each pass of up to 64 rows.  16-byte unit u of row r lies
+  // in place u ^ (r & 7 or 15): the writes (16 rows each) start in different banks.
+  constexpr int TN = BN / WN, UPR = TN / 4, FIT = NBUF * STAGE / (WM * WN * 16 * TN * 4), W = 8, LPR = TN / W;
   constexpr int PASS = FM <= FIT ? FM : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
   static_assert(FIT >= 1 && FM % PASS == 0, "whole passes that fit the stage buffers");
   float* mine = (float*)lds + wave * (PASS * 16 * TN);
+  const int cu = lane % LPR, c = j0 + wn * TN + cu * W;
+  Epilogue<T, W> epi;
+  epi.init(p, c);
 #pragma unroll
   for (int h = 0; h < FM / PASS; ++h) {
 #pragma unroll
     for (int i = 0; i < PASS; ++i)
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        const int r = i * 16 + (lane & 15), u = (j * 4 + (lane >> 4)) ^ (r & (UPR - 1));
+        const int r = i * 16 + (lane & 15), u = (j * 4 + (lane >> 4)) ^ (r & (UPR - 1) & 15);
         *(f32x4*)(mine + r * TN + u * 4) = acc[h * PASS + i][j];
       }
     // (a wave reads what itself has written: no barrier)
-    constexpr int ROWS = 64 / UPR;
+    constexpr int ROWS = 64 / LPR;
 #pragma unroll 1
     for (int r0 = 0; r0 < PASS * 16; r0 += ROWS) {
-      const int r = r0 + lane / UPR, u = lane % UPR;
-      const f32x4 v = *(const f32x4*)(mine + r * TN + ((u ^ (r & (UPR - 1))) * 4));
+      const int r = r0 + lane / LPR, sw = r & (UPR - 1) & 15;
+      const f32x4 v0 = *(const f32x4*)(mine + r * TN + ((2 * cu) ^ sw) * 4);
+      const f32x4 v1 = *(const f32x4*)(mine + r * TN + ((2 * cu + 1) ^ sw) * 4);
       const int64_t row = i0 + (wm * FM + h * PASS) * 16 + r;
-      const int c = j0 + wn * TN + u * 4;
-      if (row >= p.m || c >= p.n) continue;
-      const float d[4] = {v[0], v[1], v[2], v[3]};
+      if (row >= p.m || epi.count <= 0) continue;
+      const float d[W] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
       if (p.splits > 1) {   // (rows of the slabs are padded to whole vectors)
-        *(float4*)(p.slabs + split * p.slab_stride + row * p.slab_ld + c) = make_float4(d[0], d[1], d[2], d[3]);
+        float* slab = p.slabs + split * p.slab_stride + row * p.slab_ld + c;
+        *(float4*)slab = make_float4(d[0], d[1], d[2], d[3]);
+        *(float4*)(slab + 4) = make_float4(d[4], d[5], d[6], d[7]);
       } else {
-        linear_epilogue<T>(p, row, c, d);
+        epi.row(p, row, c, d);
       }
     }
   }
 }
 
-// Copies one or two operands into rows of whole 16-byte units, zeros behind their ends: a unit per
-// thread.
+// Up to 16 rows (the tokens of a generation step, one observation): a workgroup has 32 columns and
+// the whole depth, its eight waves take its stages in turn, each through a ring of its own -- no barrier
+// until the waves' sums meet in LDS, no slabs, one launch.  Bound by the weight's bytes: 64 KB of them
+// are on their way in each CU.
+constexpr int kRowsWaves = 8, kRowsBuffers = 3, kRowsM = 16, kRowsN = 32;
+template <typename T, bool B_KC>
+__global__ __launch_bounds__(64 * kRowsWaves) void linear_rows_kernel(DzGemmArgs p) {
+  constexpr int BK = 128 / sizeof(T), FN = kRowsN / 16;
+  constexpr int A_BYTES = kRowsM * 128, STAGE = (kRowsM + kRowsN) * 128, RING = kRowsBuffers * STAGE;
+  using SA = Stager<T, true, kRowsM, 64>;
+  using SB = Stager<T, B_KC, kRowsN, 64>;
+  constexpr int OUT = (kRowsBuffers - 2) * (SA::PER + SB::PER);
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int j0 = blockIdx.x * kRowsN;
+  const int whole = p.k / BK, rem = p.k % BK;
+  // this wave's whole stages: wave, wave + 8, ...; the last wave also has the one that is not whole
+  const bool tail = rem && wave == kRowsWaves - 1;
+  const int own = (whole - wave + kRowsWaves - 1) / kRowsWaves, stages = own + tail;
+  char* ring = lds + wave * RING;
+  const unsigned lds0 = (unsigned)(uintptr_t)ring;
+
+  f32x4 acc[FN] = {};
+  SA ra;
+  SB rb;
+  ra.init((const T*)p.a, p.lda, 0, p.m, 0, 0, lane);
+  rb.init((const T*)p.b, p.ldb, j0, p.n, 0, 0, lane);
+  const char* a0 = ra.base;
+  const char* b0 = rb.base;
+  int next = wave;
+  auto fetch = [&](int n, int buf) {   // stage n of this wave
+    const unsigned at = lds0 + buf * STAGE;
+    if (tail && n == 0) {
+      ra.base = a0; rb.base = b0;
+      ra.issue_tail(at, 0, lane, rem, whole);
+      rb.issue_tail(at + A_BYTES, 0, lane, rem, whole);
+    } else {
+      ra.base = a0 + next * ra.stage_bytes;
+      rb.base = b0 + next * rb.stage_bytes;
+      next += kRowsWaves;
+      ra.issue(at, 0);
+      rb.issue(at + A_BYTES, 0);
+    }
+  };
+#pragma unroll
+  for (int n = 0; n < kRowsBuffers - 1; ++n)
+    if (n < stages) fetch(n, n);
+  auto step = [&](int t, int buf) {
+    // the next buffer's reads are done (their products are issued), stage t is here
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (t + kRowsBuffers - 1 < stages) {
+      fetch(t + kRowsBuffers - 1, (buf + kRowsBuffers - 1) % kRowsBuffers);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OUT + SA::PER + SB::PER) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    char* sa = ring + buf * STAGE;
+    if (tail && t == 0) {
+      SA::zero_tail(sa, 0, lane, rem);
+      SB::zero_tail(sa + A_BYTES, 0, lane, rem);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const auto fa = Operand<T, true, kRowsM>::fragment(sa, 0, s, lane);
+#pragma unroll
+      for (int f = 0; f < FN; ++f)
+        acc[f] = mfma16(Operand<T, B_KC, kRowsN>::fragment(sa + A_BYTES, f, s, lane), fa, acc[f]);
+    }
+  };
+  int t = 0;
+  for (; t + kRowsBuffers <= stages; t += kRowsBuffers) {
+#pragma unroll
+    for (int n = 0; n < kRowsBuffers; ++n) step(t + n, n);
+  }
+#pragma unroll
+  for (int n = 0; n < kRowsBuffers - 1; ++n)
+    if (t + n < stages) step(t + n, n);
+
+  __syncthreads();
+  float* sums = (float*)lds;   // [wave][row][column]
+#pragma unroll
+  for (int f = 0; f < FN; ++f)
+    *(f32x4*)(sums + (wave * kRowsM + (lane & 15)) * kRowsN + f * 16 + 4 * (lane >> 4)) = acc[f];
+  __syncthreads();
+  static_assert(kRowsWaves * 64 >= kRowsM * kRowsN / 4, "a thread per four columns");
+  const int row = threadIdx.x / (kRowsN / 4), c = threadIdx.x % (kRowsN / 4) * 4;
+  if (row >= p.m || row >= kRowsM || j0 + c >= p.n) return;
+  Epilogue<T, 4> epi;
+  epi.init(p, j0 + c);
+  f32x4 v = *(const f32x4*)(sums + row * kRowsN + c);
+#pragma unroll
+  for (int w = 1; w < kRowsWaves; ++w) v += *(const f32x4*)(sums + (w * kRowsM + row) * kRowsN + c);
+  const float d[4] = {v[0], v[1], v[2], v[3]};
+  epi.row(p, row, j0 + c, d);
+}
+
+// Copies one or two operands into rows of whole 16-byte units, zeros behind their ends: 64 threads
+// along a row, four rows.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_pack_kernel(DzPackArgs p) {
   constexpr int VE = 16 / sizeof(T);
-  const DzPackArgs::One q = blockIdx.y ? p.two : p.one;
-  const int64_t per_row = q.ldd / VE, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= per_row * q.rows) return;
-  const int64_t row = id / per_row;
-  const int c = (int)(id - row * per_row) * VE;
-  const T* x = (const T*)q.src + row * q.ld + c;
-  DzPack<T, VE> v;
-  if (c + VE <= q.cols) {
-    v = dz_load<T, VE>(x);
-  } else {
+  const DzPackArgs::One q = blockIdx.z ? p.two : p.one;
+  const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * VE;
+  if (c >= q.cols) return;
+  for (int64_t row = blockIdx.y * 4 + (threadIdx.x >> 6); row < q.rows; row += gridDim.y * 4) {
+    const T* x = (const T*)q.src + row * q.ld + c;
+    DzPack<T, VE> v;
+    if (c + VE <= q.cols) {
+      v = dz_load<T, VE>(x);
+    } else {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) v.v[e] = c + e < q.cols ? x[e] : (T)0.0f;
+      for (int e = 0; e < VE; ++e) v.v[e] = c + e < q.cols ? x[e] : (T)0.0f;
+    }
+    dz_store<T, VE>((T*)q.dst + row * q.ldd + c, v);
   }
-  dz_store<T, VE>((T*)q.dst + row * q.ldd + c, v);
 }
 
-// The splits' slabs, added in order, and the epilogue: four columns per thread.
+// The splits' slabs, added in order, and the epilogue: four columns per thread, 64 threads along a
+// row.
 template <typename T>
-__global__ __launch_bounds__(256) void linear_finish_kernel(DzGemmArgs p) {
-  const int64_t per_row = p.slab_ld / 4, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= per_row * p.m) return;
-  const int64_t row = id / per_row;
-  const int c = (int)(id - row * per_row) * 4;
+__global__ __launch_bounds__(64) void linear_finish_kernel(DzGemmArgs p) {
+  const int c = (blockIdx.x * 64 + threadIdx.x) * 4;
   if (c >= p.n) return;
-  const float* at = p.slabs + row * p.slab_ld + c;
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = 0; k < p.splits; k += 8) {   // eight loads in flight; the sums in order
-    float4 x[8];
+  Epilogue<T, 4> epi;
+  epi.init(p, c);
+  for (int64_t row = blockIdx.y; row < p.m; row += gridDim.y) {
+    const float* at = p.slabs + row * p.slab_ld + c;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < p.splits; k += 8) {   // eight loads in flight; the sums in order
+      float4 x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = *(const float4*)(at + min(k + e, p.splits - 1) * p.slab_stride);
+      for (int e = 0; e < 8; ++e) x[e] = *(const float4*)(at + min(k + e, p.splits - 1) * p.slab_stride);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (k + e >= p.splits) break;
-      s.x += x[e].x; s.y += x[e].y; s.z += x[e].z; s.w += x[e].w;
+      for (int e = 0; e < 8; ++e) {
+        if (k + e >= p.splits) break;
+        s.x += x[e].x; s.y += x[e].y; s.z += x[e].z; s.w += x[e].w;
+      }
     }
+    const float d[4] = {s.x, s.y, s.z, s.w};
+    epi.row(p, row, c, d);
   }
-  const float d[4] = {s.x, s.y, s.z, s.w};
-  linear_epilogue<T>(p, row, c, d);
 }
 
 template <typename T>
@@ -424,7 +601,7 @@ __global__ __launch_bounds__(256) void linear_dact_kernel(DzDactArgs p) {
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
       y[e] = (float)d.v[e];
-      if (p.z) y[e] *= linear_act_slope((float)z.v[e], p.activation);
+      if (p.z) y[e] *= linear_act_slope<T>((float)z.v[e], p.activation);
       s[e] += y[e];
     }
     if (!p.dz) return;
@@ -441,17 +618,18 @@ __global__ __launch_bounds__(256) void linear_dact_kernel(DzDactArgs p) {
   const T* dy = (const T*)p.dy + c;
   const T* z = (const T*)p.z + c;
   if (count == VE) {
-    for (int64_t i = first + r; i < end; i += 8) {   // two rows in flight
-      const bool two = i + 4 < end;
-      const int64_t j = two ? i + 4 : i;
-      DzPack<T, VE> z0, z1;
-      const auto d0 = dz_load<T, VE>(dy + i * p.ldy), d1 = dz_load<T, VE>(dy + j * p.ldy);
-      if (p.z) {
-        z0 = dz_load<T, VE>(z + i * p.ldz);
-        z1 = dz_load<T, VE>(z + j * p.ldz);
+    constexpr int FLY = 4;   // rows in flight
+    for (int64_t i = first + r; i < end; i += 4 * FLY) {
+      DzPack<T, VE> d[FLY], zv[FLY];
+#pragma unroll
+      for (int f = 0; f < FLY; ++f) {
+        const int64_t j = min(i + 4 * f, end - 1);
+        d[f] = dz_load<T, VE>(dy + j * p.ldy);
+        if (p.z) zv[f] = dz_load<T, VE>(z + j * p.ldz);
       }
-      row(i, d0, z0);
-      if (two) row(j, d1, z1);
+#pragma unroll
+      for (int f = 0; f < FLY; ++f)
+        if (i + 4 * f < end) row(i + 4 * f, d[f], zv[f]);
     }
   } else if (count > 0) {
     for (int64_t i = first + r; i < end; i += 4) {
@@ -480,21 +658,27 @@ __global__ __launch_bounds__(256) void linear_dact_kernel(DzDactArgs p) {
   }
 }
 
-// The chunks' sums, in order.
+// The chunks' sums: 64 columns and four runs of chunks per workgroup, each in order.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_db_kernel(const float* __restrict__ sums, int chunks, int n, void* db,
                                                         int db_f32) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6, run = (chunks + 3) / 4;
+  const int first = part * run, end = min(chunks, first + run);
   float s = 0.f;
-  for (int i = 0; i < chunks; i += 8) {   // eight loads in flight; the sums in order
-    float x[8];
+  if (c < n)
+    for (int i = first; i < end; i += 8) {   // eight loads in flight
+      float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = sums[(int64_t)min(i + e, chunks - 1) * n + c];
+      for (int e = 0; e < 8; ++e) x[e] = sums[(int64_t)min(i + e, end - 1) * n + c];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (i + e < chunks) s += x[e];
-  }
+      for (int e = 0; e < 8; ++e)
+        if (i + e < end) s += x[e];
+    }
+  __shared__ float red[4][64];
+  red[part][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (part || c >= n) return;
+  s = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
   if (db_f32) ((float*)db)[c] = s;
   else ((T*)db)[c] = (T)s;
 }
