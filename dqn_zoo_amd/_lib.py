@@ -453,7 +453,7 @@ def gpu_index(name, t):
 _raw_capture = False
 
 
-def scratch(nbytes, device_index, workspace):
+def scratch(nbytes, device, workspace):
   """An operator's workspace: the caller's `workspace` (a contiguous uint8 tensor, checked) or a
   block of torch's allocator on the current stream."""
   import torch
@@ -461,8 +461,8 @@ def scratch(nbytes, device_index, workspace):
     if _raw_capture:
       raise RuntimeError('inside capture_graph the operators need the caller\'s workspace= and '
                          'output buffers: they must live as long as the graph')
-    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=torch.device('cuda', device_index))
-  if gpu_index('workspace', workspace) != device_index:
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+  if gpu_index('workspace', workspace) != device.index:
     raise ValueError('workspace is on another device')
   if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
     raise TypeError('workspace must be a contiguous uint8 tensor')

@@ -9,23 +9,29 @@
 //   d loss / d x_j = w / norm ( s (1[j = a] - p_j) + ent p_j (log p_j + H) ),
 //   s = -rho A [rho A <= clip(rho) A] - kl (exp(d) - 1)
 //
-// Everything runs in base 2: with u_j = (x_j - max x) log2 e (the difference first: log2 e times the
-// lowest float32, a common mask, is -inf), e_j = 2^u_j, S = sum e and T = sum e u give l and H.  A
-// gradient element is
-//   p_j (k1 u_j + k0) (+ s at j = a),   k1 = ent ln2,  k0 = ent (H - l) - s
-// -- one exponential and five other operations.  u is held above -200 (2^-200 is 0 in float32), so
-// that a masked logit (-inf, or the type's lowest value) gives 0 and not 0 * inf.  A row in which
-// every logit is -inf, or one is NaN or +inf, is NaN, as its log-softmax is; a row of weight 0 is
-// not read.
+// log p_j + H = t_j - mean of t, so that a gradient element is p_j (ent (t_j - mean t) - s), and at
+// j = a, s more.  Rows held by a team run in base 2: with c = log2 e, u_j = c x_j - c max x is one
+// fused multiply-add, e_j = 2^u_j; c max x is rounded, the same for every element, and what the
+// rounding left (one more fused multiply-add a row) is taken out of log sum e.  A gradient element is
+//   e_j (k1 u_j + k0),   k1 = ent ln2 / S,  k0 = (-ent mean t - s) / S,
+// times the row's factor: one exponential and five other operations an element and pass.  u is held
+// above -200 (2^-200 is 0 in float32), so that a masked logit (-inf, or the type's lowest value)
+// gives 0 and not 0 * inf.  A row whose maximum is beyond 10^38 (every logit the lowest value)
+// takes x - max first: c max overflows there.  A row in which every logit is -inf, or one is NaN or
+// +inf, is NaN, as its log-softmax is: its maximum is not finite (the maxima keep NaN); a row of
+// weight 0 is not read.
 //
 // Bound: bytes (the logits in and the gradient out).  Four forms by the size of a row:
-//   * few: 4 - 64 lanes to a row, 4 elements a lane (up to 256 logits: actions).  One workgroup does
+//   * few: 1 - 32 lanes to a row, 8 elements a lane (up to 256 logits: actions; the row's own terms,
+//     a hundred instructions, are what is to be shared by rows).  One workgroup does
 //     a small problem, weights' sum and loss included, in one launch;
 //   * team: 64, 256 or 1024 threads hold the row in registers, 1 - 16 16-byte vectors each;
 //   * split: rows that are longer than a workgroup's registers, or too few of them to fill the chip:
 //     pieces of a row are reduced by one launch and turned into the gradient by the next, for as
 //     many rows at a time as the 256 MB Infinity Cache holds, so that the second read stays on it.
 // The rows' values are summed in double in a fixed order.
+#include <type_traits>
+
 #include "dz_elem.h"
 
 namespace {
@@ -50,14 +56,19 @@ struct LossArgs {
 struct RowSums { float top, s, t; };   // max x, sum e, sum e u  (u relative to top)
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-// (a comparison, not a maximum: NaN stays)
-__device__ __forceinline__ float held(float u) { return u < -200.0f ? -200.0f : u; }
-__device__ __forceinline__ float unit(float x, float top) { return held((x - top) * kLog2e); }
+__device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }   // NaN stays
+__device__ __forceinline__ bool huge(float top) { return !(fabsf(top) < 1e38f); }
+__device__ __forceinline__ float held(float u) { return fmaxf(u, -200.0f); }
+// u of x in a row of maximum `top`: FAR where top is huge
+template <bool FAR>
+__device__ __forceinline__ float unit(float x, float top) {
+  return held(FAR ? (x - top) * kLog2e : __builtin_fmaf(x, kLog2e, -(top * kLog2e)));
+}
 
 template <int W>
 __device__ __forceinline__ float lanes_max(float x) {
 #pragma unroll
-  for (int o = W / 2; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+  for (int o = W / 2; o; o >>= 1) x = maximum(x, __shfl_xor(x, o));
   return x;
 }
 template <int W>
@@ -73,24 +84,28 @@ __device__ __forceinline__ double wave_sum_f64(double x) {
 }
 
 // `part` in units of the whole row's maximum (a part of masked logits alone adds 0: f is held too).
+// The rounded products are subtracted, as the elements' u were formed.
 __device__ __forceinline__ void rescale(RowSums& part, float top) {
-  const float f = unit(part.top, top), g = exp2_fast(f);
+  const float f = held(huge(top) ? (part.top - top) * kLog2e : part.top * kLog2e - top * kLog2e);
+  const float g = exp2_fast(f);
   part.t = g * __builtin_fmaf(part.s, f, part.t);
   part.s = g * part.s;
 }
-// the maximum that a part's sums are taken against: 0 stands in for -inf, where every e is 0
-__device__ __forceinline__ float against(float top) { return top == -__builtin_inff() ? 0.0f : top; }
 
-struct RowOut { float value, logp, entropy, slope, k1, k0, inv_s; };
+// what the rounding of c * top left: u = c (x - top) + residue
+__device__ __forceinline__ float residue(float top) {
+  return huge(top) ? 0.0f : __builtin_fmaf(top, kLog2e, -(top * kLog2e));
+}
 
-__device__ __forceinline__ RowOut row_values(const LossArgs& a, const RowSums& r, float xa, float adv,
+struct RowOut { float value, logp, entropy, slope; };
+
+// `lse`: log sum exp t; `mean`: of t; both of the natural t = x - top
+__device__ __forceinline__ RowOut row_values(const LossArgs& a, float top, float lse, float mean, float xa, float adv,
                                              float old, float ref) {
   RowOut o;
-  const float log2s = __builtin_amdgcn_logf(r.s);   // (base 2)
-  o.inv_s = 1.0f / r.s;
-  o.logp = (xa - r.top) - log2s * kLn2;
-  const float mean_u = r.t * o.inv_s;
-  o.entropy = (log2s - mean_u) * kLn2;
+  if (!(fabsf(top) < __builtin_inff())) lse = __builtin_nanf("");
+  o.logp = (xa - top) - lse;
+  o.entropy = lse - mean;
   const float rho = expf(o.logp - old);
   const float free = rho * adv;
   // (1 - lo and 1 + hi are formed in double on the host)
@@ -104,15 +119,25 @@ __device__ __forceinline__ RowOut row_values(const LossArgs& a, const RowSums& r
     o.slope = __builtin_fmaf(-a.kl, e, o.slope);
   }
   o.value = __builtin_fmaf(-a.ent, o.entropy, o.value);
-  o.k1 = a.ent * kLn2;
-  o.k0 = __builtin_fmaf(a.ent, -mean_u * kLn2, -o.slope);   // H - l = -mean_u ln 2
+  return o;
+}
+// of a row in base 2; k1 and k0 are the gradient's, without the row's factor
+__device__ __forceinline__ RowOut row_values(const LossArgs& a, const RowSums& r, float xa, float adv, float old,
+                                             float ref, float& k1, float& k0) {
+  const float inv_s = 1.0f / r.s, left = residue(r.top);
+  const float mean = (r.t * inv_s - left) * kLn2;
+  const RowOut o = row_values(a, r.top, logf(r.s) - left * kLn2, mean, xa, adv, old, ref);
+  const float none = fabsf(r.top) < __builtin_inff() ? inv_s : __builtin_nanf("");
+  k1 = a.ent * kLn2 * none;
+  k0 = (__builtin_fmaf(-a.ent, mean + left * kLn2, -o.slope)) * none;
   return o;
 }
 
-// d loss / d x_j without the row's factor and without the action's own term
-__device__ __forceinline__ float gradient(float x, const RowSums& r, const RowOut& o, float factor) {
-  const float u = unit(x, r.top);
-  return (exp2_fast(u) * o.inv_s) * (__builtin_fmaf(o.k1, u, o.k0) * factor);
+// d loss / d x_j without the action's own term; k1 and k0 have the row's factor
+template <bool FAR>
+__device__ __forceinline__ float gradient(float x, float top, float k1, float k0) {
+  const float u = unit<FAR>(x, top);
+  return exp2_fast(u) * __builtin_fmaf(k1, u, k0);
 }
 
 __device__ __forceinline__ double inverse_norm(const LossArgs& a) {   // (whole waves)
@@ -167,10 +192,11 @@ __global__ __launch_bounds__(1024) void loss_total_kernel(LossArgs a, int64_t n)
 }
 
 // ---- few: G lanes to a row --------------------------------------------------
-// ALL: the one workgroup takes every row in turn, and the weights' sum and the loss with them.
+// ALL: the one workgroup takes every row in turn, and the weights' sum and the loss with them.  (In
+// natural units and with the library's functions: nothing here is bound by the elements.)
 template <typename T, int G, bool ALL>
 __global__ __launch_bounds__(256) void loss_few_kernel(LossArgs a) {
-  constexpr int E = 4, ROWS = 256 / G;
+  constexpr int E = 8, ROWS = 256 / G;
   const int lane = threadIdx.x % G;
   __shared__ double red[4];
   double inv, total = 0.0;
@@ -194,26 +220,27 @@ __global__ __launch_bounds__(256) void loss_few_kernel(LossArgs a) {
     const bool used = live && in.w != 0.0f;
     const T* x = (const T*)a.logits + row * a.ld;
     float v[E];
-    float m = -__builtin_inff();
+    float top = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       const int c = j * G + lane;
       v[j] = used && c < a.classes ? (float)x[c] : -__builtin_inff();
-      m = fmaxf(m, v[j]);
+      top = maximum(top, v[j]);
     }
-    RowSums r;
-    r.top = lanes_max<G>(m);
-    const float top = against(r.top);
-    r.s = r.t = 0.f;
+    top = lanes_max<G>(top);
+    float s = 0.f, t = 0.f;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      const float u = unit(v[j], top), e = exp2_fast(u);
-      r.s += e;
-      r.t = __builtin_fmaf(e, u, r.t);
+      if (j * G >= a.classes) break;   // (uniform)
+      const float d = fmaxf(v[j] - top, -200.0f), e = expf(d);
+      v[j] = d;
+      s += e;
+      t = __builtin_fmaf(e, d, t);
     }
-    r.s = lanes_sum<G>(r.s);
-    r.t = lanes_sum<G>(r.t);
-    const RowOut o = row_values(a, r, in.xa, in.adv, in.old, in.ref);
+    s = lanes_sum<G>(s);
+    t = lanes_sum<G>(t);
+    const float mean = t / s;
+    const RowOut o = row_values(a, top, logf(s), mean, in.xa, in.adv, in.old, in.ref);
     const float factor = (float)(used ? (double)in.w * inv * (double)a.grad_scale : 0.0);
     if (live && lane == 0) {
       a.logp[row] = used ? o.logp : 0.0f;
@@ -222,13 +249,14 @@ __global__ __launch_bounds__(256) void loss_few_kernel(LossArgs a) {
     }
     if (a.grad && live) {
       T* g = (T*)a.grad + row * a.ldg;
+      const float inv_s = fabsf(top) < __builtin_inff() ? 1.0f / s : __builtin_nanf("");
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const int c = j * G + lane;
         if (c >= a.classes) continue;
-        float y = used ? gradient(v[j], r, o, factor) : 0.0f;
-        if (used && c == in.action) y += o.slope * factor;
-        g[c] = (T)y;
+        float y = expf(v[j]) * inv_s * (__builtin_fmaf(a.ent, v[j] - mean, -o.slope) * factor);
+        if (c == in.action) y += o.slope * factor;
+        g[c] = (T)(used ? y : 0.0f);
       }
     }
   }
@@ -243,11 +271,43 @@ __global__ __launch_bounds__(256) void loss_few_kernel(LossArgs a) {
 }
 
 // ---- team: TEAM threads hold a row -------------------------------------------
+// A thread's part of a row, as it lies in memory.  `forget` between the passes: the compiler would
+// keep the float32 values of the first for the second, twice the registers (8 vectors of bf16 in
+// 1024 threads: 111 registers against 56, so one workgroup per CU and not two; 16 vectors spill).
 template <typename T, int NV>
 struct RowRegs {
   static constexpr int VE = 16 / sizeof(T);
-  DzPack<T, VE> v[NV];
+  typedef __attribute__((ext_vector_type(4))) uint32_t Words;
+  Words w[NV];
+
+  template <int PLACE>   // (another text at each place: equal ones of two branches would be hoisted)
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) asm volatile("; pass %1" : "+v"(w[i]) : "n"(PLACE));
+  }
+  __device__ __forceinline__ DzPack<T, VE> get(int i) const { return __builtin_bit_cast(DzPack<T, VE>, w[i]); }
+  __device__ __forceinline__ float at(int i, int j) const { return (float)get(i).v[j]; }
 };
+
+// The 16 bytes from element c of a row of n that end behind it: what is there, and -inf (a rolled
+// loop: one thread of a row has such a vector, and eight two-byte loads each would cost registers).
+template <typename T>
+__device__ __forceinline__ typename RowRegs<T, 1>::Words row_end(const T* x, int c, int n) {
+  typedef std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t> Raw;
+  const uint64_t none = __builtin_bit_cast(Raw, (T)-__builtin_inff());
+  const uint64_t fill = sizeof(T) == 2 ? none * 0x0001000100010001ull : none * 0x0000000100000001ull;
+  uint64_t q[2] = {fill, fill};
+#pragma unroll 1
+  for (int j = 0; c + j < n; ++j) {
+    const int bit = j * 8 * (int)sizeof(T);
+    const uint64_t flip = (none ^ (uint64_t)__builtin_bit_cast(Raw, x[c + j])) << (bit & 63);
+    q[0] ^= bit < 64 ? flip : 0;
+    q[1] ^= bit < 64 ? 0 : flip;
+  }
+  typename RowRegs<T, 1>::Words w;
+  w[0] = (uint32_t)q[0]; w[1] = (uint32_t)(q[0] >> 32); w[2] = (uint32_t)q[1]; w[3] = (uint32_t)(q[1] >> 32);
+  return w;
+}
 
 // vector i of thread t is vector i * TEAM + t of the row; what is past the row is -inf
 template <typename T, int TEAM, int NV>
@@ -256,54 +316,58 @@ __device__ __forceinline__ void load_row(const T* x, int n, int tid, RowRegs<T, 
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * TEAM + tid) * VE;
-    if (c + VE <= n) {
-      r.v[i] = dz_load<T, VE>(x + c);
-    } else {
+    r.w[i] = c + VE <= n ? __builtin_bit_cast(typename RowRegs<T, NV>::Words, dz_load<T, VE>(x + c)) : row_end<T>(x, c, n);
+  }
+}
+
+template <bool FAR, typename T, int NV>
+__device__ __forceinline__ void sum_exponentials(RowRegs<T, NV>& r, RowSums& o) {
+  r.template forget<FAR>();
 #pragma unroll
-      for (int j = 0; j < VE; ++j) r.v[i].v[j] = c + j < n ? x[c + j] : (T)-__builtin_inff();
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < 16 / (int)sizeof(T); ++j) {
+      const float u = unit<FAR>(r.at(i, j), o.top), e = exp2_fast(u);
+      o.s += e;
+      o.t = __builtin_fmaf(e, u, o.t);
     }
+    __builtin_amdgcn_sched_barrier(0);   // (one vector's values at a time: registers)
   }
 }
 
 template <typename T, int NV>
-__device__ __forceinline__ RowSums sum_row(const RowRegs<T, NV>& r) {   // one wave's part
-  constexpr int VE = 16 / sizeof(T);
+__device__ __forceinline__ RowSums sum_row(RowRegs<T, NV>& r) {   // one wave's part
   float m = -__builtin_inff();
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
 #pragma unroll
-    for (int j = 0; j < VE; ++j) m = fmaxf(m, (float)r.v[i].v[j]);
-  RowSums o;
-  o.top = lanes_max<64>(m);
-  const float top = against(o.top);
-  o.s = o.t = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      const float u = unit((float)r.v[i].v[j], top), e = exp2_fast(u);
-      o.s += e;
-      o.t = __builtin_fmaf(e, u, o.t);
-    }
+    for (int j = 0; j < 16 / (int)sizeof(T); ++j) m = maximum(m, r.at(i, j));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  RowSums o{lanes_max<64>(m), 0.f, 0.f};
+  if (huge(o.top)) sum_exponentials<true>(r, o);
+  else sum_exponentials<false>(r, o);
   o.s = lanes_sum<64>(o.s);
   o.t = lanes_sum<64>(o.t);
   return o;
 }
 
-template <typename T, int TEAM, int NV>
-__device__ __forceinline__ void store_gradient(T* g, int n, int tid, const RowRegs<T, NV>& x, const RowSums& r,
-                                               const RowOut& o, float factor, int64_t action, bool used) {
+template <bool FAR, typename T, int TEAM, int NV>
+__device__ __forceinline__ void store_rows(T* g, int n, int tid, RowRegs<T, NV>& x, float top, float k1, float k0,
+                                           float own, int64_t action) {
   constexpr int VE = 16 / sizeof(T);
+  x.template forget<2 + FAR>();
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * TEAM + tid) * VE;
+    if (c >= n) break;
     float y[VE];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) y[j] = used ? gradient((float)x.v[i].v[j], r, o, factor) : 0.0f;
-    if (used && action >= c && action < c + VE) {
+    for (int j = 0; j < VE; ++j) y[j] = gradient<FAR>(x.at(i, j), top, k1, k0);
+    if (action >= c && action < c + VE) {
 #pragma unroll
       for (int j = 0; j < VE; ++j)
-        if (c + j == action) y[j] += o.slope * factor;
+        if (c + j == action) y[j] += own;
     }
     if (c + VE <= n) {
       dz_store<T, VE>(g + c, dz_round<T, VE>(y));
@@ -312,11 +376,41 @@ __device__ __forceinline__ void store_gradient(T* g, int n, int tid, const RowRe
       for (int j = 0; j < VE; ++j)
         if (c + j < n) g[c + j] = (T)y[j];
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
 template <typename T, int TEAM, int NV>
-__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void loss_team_kernel(LossArgs a) {
+__device__ __forceinline__ void store_gradient(T* g, int n, int tid, RowRegs<T, NV>& x, const RowSums& r,
+                                               const RowOut& o, float k1, float k0, float factor, int64_t action,
+                                               bool used) {
+  constexpr int VE = 16 / sizeof(T);
+  if (!used) {
+    DzPack<T, VE> zero;
+#pragma unroll
+    for (int j = 0; j < VE; ++j) zero.v[j] = (T)0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TEAM + tid) * VE;
+      if (c + VE <= n) {
+        dz_store<T, VE>(g + c, zero);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+          if (c + j < n) g[c + j] = (T)0.0f;
+      }
+    }
+    return;
+  }
+  k1 *= factor;
+  k0 *= factor;
+  const float own = o.slope * factor;
+  if (huge(r.top)) store_rows<true, T, TEAM, NV>(g, n, tid, x, r.top, k1, k0, own, action);
+  else store_rows<false, T, TEAM, NV>(g, n, tid, x, r.top, k1, k0, own, action);
+}
+
+template <typename T, int TEAM, int NV>
+__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM, NV <= 8 ? 8 : 4) void loss_team_kernel(LossArgs a) {
   constexpr int THREADS = TEAM < 256 ? 256 : TEAM, PER = THREADS / TEAM, WAVES = TEAM / 64;
   const int tid = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
   const int64_t row = (int64_t)blockIdx.x * PER + team;
@@ -339,16 +433,16 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void loss_team_kernel(Loss
     // lane k of every wave takes part k
     const int k = threadIdx.x & 63;
     RowSums q = k < WAVES ? parts[k] : RowSums{-__builtin_inff(), 0.f, 0.f};
-    r.top = lanes_max<WAVES>(q.top);
-    r.top = __shfl(r.top, 0);
+    r.top = __shfl(lanes_max<WAVES>(q.top), 0);
     rescale(q, r.top);
     r.s = __shfl(lanes_sum<WAVES>(q.s), 0);
     r.t = __shfl(lanes_sum<WAVES>(q.t), 0);
   }
-  const RowOut o = row_values(a, r, in.xa, in.adv, in.old, in.ref);
+  float k1, k0;
+  const RowOut o = row_values(a, r, in.xa, in.adv, in.old, in.ref, k1, k0);
   const float factor = (float)(used ? (double)in.w * inv * (double)a.grad_scale : 0.0);
   if (a.grad && live)
-    store_gradient<T, TEAM, NV>((T*)a.grad + row * a.ldg, a.classes, tid, x, r, o, factor, in.action, used);
+    store_gradient<T, TEAM, NV>((T*)a.grad + row * a.ldg, a.classes, tid, x, r, o, k1, k0, factor, in.action, used);
   if (tid == 0) {
     if (live) {
       a.logp[row] = used ? o.logp : 0.0f;
@@ -384,7 +478,7 @@ __global__ __launch_bounds__(256) void loss_split_sums_kernel(LossArgs a, SplitW
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = q;
   __syncthreads();
   if (threadIdx.x) return;
-  RowSums r{fmaxf(fmaxf(red[0].top, red[1].top), fmaxf(red[2].top, red[3].top)), 0.f, 0.f};
+  RowSums r{maximum(maximum(red[0].top, red[1].top), maximum(red[2].top, red[3].top)), 0.f, 0.f};
   for (int i = 0; i < 4; ++i) {
     q = red[i];
     rescale(q, r.top);
@@ -405,12 +499,13 @@ __global__ __launch_bounds__(256) void loss_split_gradient_kernel(LossArgs a, Sp
   const int n = min(a.classes - c0, split_piece<T>());
   RowSums r{0.f, 1.f, 0.f};
   RowOut o{};
+  float k1 = 0.f, k0 = 0.f;
   int64_t action = a.actions[row];
   if (used) {
     if (a.grad) load_row<T, 256, kSplitVectors>((const T*)a.logits + row * a.ld + c0, n, threadIdx.x, x);
     const RowSums* parts = ws.parts + local * ws.pieces;   // every wave folds the row's parts, in one order
     float top = -__builtin_inff();
-    for (int i = threadIdx.x & 63; i < ws.pieces; i += 64) top = fmaxf(top, parts[i].top);
+    for (int i = threadIdx.x & 63; i < ws.pieces; i += 64) top = maximum(top, parts[i].top);
     r.top = lanes_max<64>(top);
     r.s = r.t = 0.f;
     for (int i = threadIdx.x & 63; i < ws.pieces; i += 64) {
@@ -421,12 +516,13 @@ __global__ __launch_bounds__(256) void loss_split_gradient_kernel(LossArgs a, Sp
     }
     r.s = lanes_sum<64>(r.s);
     r.t = lanes_sum<64>(r.t);
-    o = row_values(a, r, ws.xa[local], a.advantages[row], a.old_logp[row], a.ref_logp ? a.ref_logp[row] : 0.0f);
+    o = row_values(a, r, ws.xa[local], a.advantages[row], a.old_logp[row], a.ref_logp ? a.ref_logp[row] : 0.0f, k1,
+                   k0);
   }
   const float factor = (float)(used ? (double)w * inv * (double)a.grad_scale : 0.0);
   if (a.grad)
-    store_gradient<T, 256, kSplitVectors>((T*)a.grad + row * a.ldg + c0, n, threadIdx.x, x, r, o, factor,
-                                          action - c0, used);
+    store_gradient<T, 256, kSplitVectors>((T*)a.grad + row * a.ldg + c0, n, threadIdx.x, x, r, o, k1, k0,
+                                          factor, action - c0, used);
   if (piece == 0 && threadIdx.x == 0) {
     a.logp[row] = used ? o.logp : 0.0f;
     a.entropy[row] = used ? o.entropy : 0.0f;
@@ -453,12 +549,12 @@ Plan make_plan(int dtype, int64_t rows, int classes) {
   const int ve = dtype == DZ_F32 ? 4 : 8;
   int64_t bytes = kWeightBlocks * 8;
   if (classes <= 256) {
-    p.lanes = 4;
-    while (p.lanes * 4 < classes) p.lanes *= 2;
+    p.lanes = 1;
+    while (p.lanes * 8 < classes) p.lanes *= 2;
     const int64_t per = 256 / p.lanes;
     p.blocks = (rows + per - 1) / per;
     p.form = p.blocks <= 2 ? Form::kOne : Form::kFew;
-    p.ws_bytes = bytes + p.blocks * 8;
+    p.ws_bytes = p.form == Form::kOne ? 0 : bytes + p.blocks * 8;
     return p;
   }
   const int vecs = (classes + ve - 1) / ve;
@@ -491,11 +587,12 @@ void launch_team(const LossArgs& k, unsigned grid, hipStream_t s) {
 template <typename T, bool ALL>
 void launch_few(const LossArgs& k, int lanes, unsigned grid, hipStream_t s) {
   switch (lanes) {
+    case 1: hipLaunchKernelGGL((loss_few_kernel<T, 1, ALL>), dim3(grid), dim3(256), 0, s, k); break;
+    case 2: hipLaunchKernelGGL((loss_few_kernel<T, 2, ALL>), dim3(grid), dim3(256), 0, s, k); break;
     case 4: hipLaunchKernelGGL((loss_few_kernel<T, 4, ALL>), dim3(grid), dim3(256), 0, s, k); break;
     case 8: hipLaunchKernelGGL((loss_few_kernel<T, 8, ALL>), dim3(grid), dim3(256), 0, s, k); break;
     case 16: hipLaunchKernelGGL((loss_few_kernel<T, 16, ALL>), dim3(grid), dim3(256), 0, s, k); break;
-    case 32: hipLaunchKernelGGL((loss_few_kernel<T, 32, ALL>), dim3(grid), dim3(256), 0, s, k); break;
-    default: hipLaunchKernelGGL((loss_few_kernel<T, 64, ALL>), dim3(grid), dim3(256), 0, s, k); break;
+    default: hipLaunchKernelGGL((loss_few_kernel<T, 32, ALL>), dim3(grid), dim3(256), 0, s, k); break;
   }
 }
 
@@ -553,12 +650,12 @@ extern "C" int dz_policy_loss_workspace(int dtype, int64_t rows, int64_t classes
 
 extern "C" int dz_policy_loss(const dz_policy_loss_args_t* a, dz_stream_t stream) {
   DZ_REQUIRE(a && sizes_ok(a->dtype, a->rows, a->classes));
-  DZ_REQUIRE(a->logits && a->actions && a->advantages && a->old_logp && a->logp && a->entropy && a->loss && a->ws);
+  DZ_REQUIRE(a->logits && a->actions && a->advantages && a->old_logp && a->logp && a->entropy && a->loss);
   DZ_REQUIRE(a->ld >= a->classes && (!a->dlogits || a->ldg >= a->classes));
   DZ_REQUIRE(((uintptr_t)a->ws & 15) == 0);
   DZ_REQUIRE(a->clip_low >= 0.0 && a->clip_high >= 0.0 && a->normalizer >= 0.0);
   const Plan p = make_plan(a->dtype, a->rows, (int)a->classes);
-  DZ_REQUIRE(a->ws_bytes >= p.ws_bytes);
+  DZ_REQUIRE(p.ws_bytes == 0 || (a->ws && a->ws_bytes >= p.ws_bytes));
   const hipStream_t s = dz_s(stream);
   double* sums = (double*)a->ws;
   const bool summed = a->weights && !(a->normalizer > 0.0);

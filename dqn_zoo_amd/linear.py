@@ -114,7 +114,7 @@ def _workspace(lib, a, backward, device, workspace):
   need = ctypes.c_int64()
   _lib.check(lib.dz_linear_workspace(ctypes.byref(a), backward, ctypes.byref(need)),
              'dz_linear_workspace')
-  if not need.value:
+  if not need.value and workspace is None:
     return None
   ws = _lib.scratch(need.value, device, workspace)
   a.ws, a.ws_bytes = ws.data_ptr(), need.value
@@ -178,7 +178,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, b: typing.Optional[torch.Tensor] = 
       a.preact = preact.data_ptr()
     a.y = out.data_ptr()
     lib = _lib.load()
-    ws = _workspace(lib, a, 0, device, workspace)  # pylint: disable=unused-variable
+    ws = _workspace(lib, a, 0, x.device, workspace)  # pylint: disable=unused-variable
     _lib.check(lib.dz_linear(ctypes.byref(a), _lib.stream_ptr(device)), 'dz_linear')
   return (out, preact) if save_preact else out
 
@@ -246,7 +246,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
         _apart('db', db, dx=dx, dw=dw, **reads)
       a.db = db.data_ptr()
     lib = _lib.load()
-    ws = _workspace(lib, a, 1, device, workspace)  # pylint: disable=unused-variable
+    ws = _workspace(lib, a, 1, x.device, workspace)  # pylint: disable=unused-variable
     _lib.check(lib.dz_linear_backward(ctypes.byref(a), _lib.stream_ptr(device)),
                'dz_linear_backward')
   return dx, dw, db

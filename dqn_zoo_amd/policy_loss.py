@@ -34,7 +34,7 @@ class PolicyLossOutputs(typing.NamedTuple):
 
 
 def workspace_bytes(rows: int, classes: int, dtype: torch.dtype) -> int:
-  """Bytes of `policy_loss`'s workspace= for these sizes."""
+  """Bytes of `policy_loss`'s workspace= for these sizes; may be 0."""
   code = _lib.dtype_code(dtype)
   if code is None:
     raise TypeError('logits must be float32, bfloat16 or float16, got %s' % dtype)
@@ -147,8 +147,12 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.T
         if (a.dlogits < a.logits + ((rows - 1) * a.ld + classes) * size and
             a.logits < a.dlogits + ((rows - 1) * a.ldg + classes) * size):
           raise ValueError('out.dlogits overlaps the logits without being them')
-    a.ws_bytes = workspace_bytes(rows, classes, logits.dtype)
-    ws = _lib.scratch(a.ws_bytes, device, workspace)
-    a.ws = ws.data_ptr()
-    _lib.check(_lib.load().dz_policy_loss(ctypes.byref(a), _lib.stream_ptr(device)), 'dz_policy_loss')
+    lib = _lib.load()
+    need = ctypes.c_int64()
+    _lib.check(lib.dz_policy_loss_workspace(code, rows, classes, ctypes.byref(need)),
+               'dz_policy_loss_workspace')
+    if need.value or workspace is not None:
+      ws = _lib.scratch(need.value, logits.device, workspace)
+      a.ws, a.ws_bytes = ws.data_ptr(), need.value
+    _lib.check(lib.dz_policy_loss(ctypes.byref(a), _lib.stream_ptr(device)), 'dz_policy_loss')
   return out

@@ -887,7 +887,7 @@ typedef struct {
   float* logp;               /* [rows]                                           */
   float* entropy;            /* [rows]                                           */
   uint32_t* status;          /* or NULL                                          */
-  void* ws; int64_t ws_bytes;  /* dz_policy_loss_workspace; 16-byte aligned, contents arbitrary */
+  void* ws; int64_t ws_bytes;  /* dz_policy_loss_workspace (may be 0); 16-byte aligned, contents arbitrary */
   double clip_low, clip_high, normalizer;
   float kl_coef, entropy_coef, grad_scale;
   int32_t reserved2;

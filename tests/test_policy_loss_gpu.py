@@ -344,7 +344,9 @@ def test_refusals():
   refused(ValueError, 'normalizer', normalizer=float('nan'))
   refused(TypeError, 'status', status=torch.zeros(1, device='cuda'))
   refused(TypeError, 'workspace', workspace=torch.zeros(4, device='cuda'))
-  refused(ValueError, 'workspace needs', workspace=torch.zeros(4, dtype=torch.uint8, device='cuda'))
+  big = _inputs(4, 9000, torch.float32, 1)
+  with pytest.raises(ValueError, match='workspace needs'):
+    pl.policy_loss(**big, workspace=torch.zeros(4, dtype=torch.uint8, device='cuda'))
   o = pl.policy_loss(**i)
   refused(ValueError, 'exactly if', out=o, with_gradient=False)
   refused(ValueError, 'exactly if', out=o._replace(dlogits=None))
