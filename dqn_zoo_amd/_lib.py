@@ -215,8 +215,8 @@ class PolicyLossArgs(ctypes.Structure):
               ('old_logp', c_vp), ('ref_logp', c_vp), ('weights', c_vp), ('dlogits', c_vp),
               ('ldg', c_i64), ('loss', c_vp), ('logp', c_vp), ('entropy', c_vp),
               ('status', c_vp), ('ws', c_vp), ('ws_bytes', c_i64), ('clip_low', c_f64),
-              ('clip_high', c_f64), ('normalizer', c_f64), ('kl_coef', c_f32),
-              ('entropy_coef', c_f32), ('grad_scale', c_f32), ('reserved2', c_i32)]
+              ('clip_high', c_f64), ('kl_coef', c_f64), ('entropy_coef', c_f64),
+              ('normalizer', c_f64), ('grad_scale', c_f32), ('reserved2', c_i32)]
 
 
 class LinearArgs(ctypes.Structure):

@@ -49,7 +49,8 @@ struct LossArgs {
   double* values;                    // one partial loss per workgroup (row in the split form)
   const double* weight_sums;         // kWeightBlocks partial sums, or NULL: inv_norm holds
   double inv_norm;
-  float low, high, kl, ent, grad_scale;
+  double low, high, kl, ent_coef;    // of the values, in double: a coefficient's rounding is the same in every row
+  float ent, grad_scale;
   int64_t rows; int classes;
 };
 
@@ -97,7 +98,11 @@ __device__ __forceinline__ float residue(float top) {
   return huge(top) ? 0.0f : __builtin_fmaf(top, kLog2e, -(top * kLog2e));
 }
 
-struct RowOut { float value, logp, entropy, slope; };
+// The sum's logarithm, once a row: logf is 5e-8 low on average, which a loss of 10^5 rows whose terms
+// cancel shows (8e-6 of it).
+__device__ __forceinline__ float log_sum(float s) { return (float)log((double)s); }
+
+struct RowOut { double value; float logp, entropy, slope; };
 
 // `lse`: log sum exp t; `mean`: of t; both of the natural t = x - top
 __device__ __forceinline__ RowOut row_values(const LossArgs& a, float top, float lse, float mean, float xa, float adv,
@@ -106,31 +111,44 @@ __device__ __forceinline__ RowOut row_values(const LossArgs& a, float top, float
   if (!(fabsf(top) < __builtin_inff())) lse = __builtin_nanf("");
   o.logp = (xa - top) - lse;
   o.entropy = lse - mean;
-  const float rho = expf(o.logp - old);
-  const float free = rho * adv;
-  // (1 - lo and 1 + hi are formed in double on the host)
-  const float kept = (rho < a.low ? a.low : rho > a.high ? a.high : rho) * adv;
+  const double rho = (double)expf(o.logp - old), free = rho * (double)adv;
+  const double kept = (rho < a.low ? a.low : rho > a.high ? a.high : rho) * (double)adv;
   o.value = -(free <= kept ? free : kept);
-  o.slope = free <= kept ? -free : 0.0f;
-  if (free != free || kept != kept) o.value = o.slope = __builtin_nanf("");
+  double slope = free <= kept ? -free : 0.0;
+  if (free != free || kept != kept) o.value = slope = __builtin_nan("");
   if (a.ref_logp) {
-    const float d = ref - o.logp, e = expm1f(d);
-    o.value = __builtin_fmaf(a.kl, e - d, o.value);
-    o.slope = __builtin_fmaf(-a.kl, e, o.slope);
+    const double d = (double)ref - (double)o.logp, e = expm1(d);
+    o.value += a.kl * (e - d);
+    slope -= a.kl * e;
   }
-  o.value = __builtin_fmaf(-a.ent, o.entropy, o.value);
+  o.value -= a.ent_coef * (double)o.entropy;
+  o.slope = (float)slope;
   return o;
 }
-// of a row in base 2; k1 and k0 are the gradient's, without the row's factor
+// The slope alone, in float32: what the gradient's threads need.
+__device__ __forceinline__ float row_slope(const LossArgs& a, float logp, float adv, float old, float ref) {
+  const float rho = expf(logp - old), free = rho * adv;
+  const float kept = (rho < (float)a.low ? (float)a.low : rho > (float)a.high ? (float)a.high : rho) * adv;
+  float slope = free <= kept ? -free : 0.0f;
+  if (free != free || kept != kept) slope = __builtin_nanf("");
+  return a.ref_logp ? __builtin_fmaf(-(float)a.kl, expm1f(ref - logp), slope) : slope;
+}
+// A row in base 2 for its gradient (k1, k0 without the row's factor; the slope) ...
+__device__ __forceinline__ float row_gradient(const LossArgs& a, const RowSums& r, float xa, float adv, float old,
+                                              float ref, float& k1, float& k0) {
+  const float inv_s = 1.0f / r.s, left = residue(r.top) * kLn2;
+  const float slope = row_slope(a, (xa - r.top) - (logf(r.s) - left), adv, old, ref);
+  const float scale = fabsf(r.top) < __builtin_inff() ? inv_s : __builtin_nanf("");
+  k1 = a.ent * kLn2 * scale;
+  k0 = __builtin_fmaf(-a.ent, r.t * inv_s * kLn2, -slope) * scale;
+  return slope;
+}
+// ... and for its value (one wave of a team: 200 instructions of double are 20 us of a 370 us launch
+// if sixteen waves do them).
 __device__ __forceinline__ RowOut row_values(const LossArgs& a, const RowSums& r, float xa, float adv, float old,
-                                             float ref, float& k1, float& k0) {
-  const float inv_s = 1.0f / r.s, left = residue(r.top);
-  const float mean = (r.t * inv_s - left) * kLn2;
-  const RowOut o = row_values(a, r.top, logf(r.s) - left * kLn2, mean, xa, adv, old, ref);
-  const float none = fabsf(r.top) < __builtin_inff() ? inv_s : __builtin_nanf("");
-  k1 = a.ent * kLn2 * none;
-  k0 = (__builtin_fmaf(-a.ent, mean + left * kLn2, -o.slope)) * none;
-  return o;
+                                             float ref) {
+  const float left = residue(r.top);
+  return row_values(a, r.top, log_sum(r.s) - left * kLn2, (r.t / r.s - left) * kLn2, xa, adv, old, ref);
 }
 
 // d loss / d x_j without the action's own term; k1 and k0 have the row's factor
@@ -240,12 +258,12 @@ __global__ __launch_bounds__(256) void loss_few_kernel(LossArgs a) {
     s = lanes_sum<G>(s);
     t = lanes_sum<G>(t);
     const float mean = t / s;
-    const RowOut o = row_values(a, top, logf(s), mean, in.xa, in.adv, in.old, in.ref);
+    const RowOut o = row_values(a, top, log_sum(s), mean, in.xa, in.adv, in.old, in.ref);
     const float factor = (float)(used ? (double)in.w * inv * (double)a.grad_scale : 0.0);
     if (live && lane == 0) {
       a.logp[row] = used ? o.logp : 0.0f;
       a.entropy[row] = used ? o.entropy : 0.0f;
-      if (used) total += (double)in.w * (double)o.value;
+      if (used) total += (double)in.w * o.value;
     }
     if (a.grad && live) {
       T* g = (T*)a.grad + row * a.ldg;
@@ -382,7 +400,7 @@ __device__ __forceinline__ void store_rows(T* g, int n, int tid, RowRegs<T, NV>&
 
 template <typename T, int TEAM, int NV>
 __device__ __forceinline__ void store_gradient(T* g, int n, int tid, RowRegs<T, NV>& x, const RowSums& r,
-                                               const RowOut& o, float k1, float k0, float factor, int64_t action,
+                                               float slope, float k1, float k0, float factor, int64_t action,
                                                bool used) {
   constexpr int VE = 16 / sizeof(T);
   if (!used) {
@@ -404,7 +422,7 @@ __device__ __forceinline__ void store_gradient(T* g, int n, int tid, RowRegs<T, 
   }
   k1 *= factor;
   k0 *= factor;
-  const float own = o.slope * factor;
+  const float own = slope * factor;
   if (huge(r.top)) store_rows<true, T, TEAM, NV>(g, n, tid, x, r.top, k1, k0, own, action);
   else store_rows<false, T, TEAM, NV>(g, n, tid, x, r.top, k1, k0, own, action);
 }
@@ -438,17 +456,21 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM, NV <= 8 ? 8 : 4) void loss
     r.s = __shfl(lanes_sum<WAVES>(q.s), 0);
     r.t = __shfl(lanes_sum<WAVES>(q.t), 0);
   }
-  float k1, k0;
-  const RowOut o = row_values(a, r, in.xa, in.adv, in.old, in.ref, k1, k0);
   const float factor = (float)(used ? (double)in.w * inv * (double)a.grad_scale : 0.0);
-  if (a.grad && live)
-    store_gradient<T, TEAM, NV>((T*)a.grad + row * a.ldg, a.classes, tid, x, r, o, k1, k0, factor, in.action, used);
-  if (tid == 0) {
-    if (live) {
-      a.logp[row] = used ? o.logp : 0.0f;
-      a.entropy[row] = used ? o.entropy : 0.0f;
+  if (a.grad && live) {
+    float k1, k0;
+    const float slope = row_gradient(a, r, in.xa, in.adv, in.old, in.ref, k1, k0);
+    store_gradient<T, TEAM, NV>((T*)a.grad + row * a.ldg, a.classes, tid, x, r, slope, k1, k0, factor, in.action, used);
+  }
+  if (tid < 64) {   // (one wave of the team)
+    const RowOut o = row_values(a, r, in.xa, in.adv, in.old, in.ref);
+    if (tid == 0) {
+      if (live) {
+        a.logp[row] = used ? o.logp : 0.0f;
+        a.entropy[row] = used ? o.entropy : 0.0f;
+      }
+      vals[team] = used ? (double)in.w * o.value : 0.0;
     }
-    vals[team] = used ? (double)in.w * (double)o.value : 0.0;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -498,8 +520,8 @@ __global__ __launch_bounds__(256) void loss_split_gradient_kernel(LossArgs a, Sp
   RowRegs<T, kSplitVectors> x;
   const int n = min(a.classes - c0, split_piece<T>());
   RowSums r{0.f, 1.f, 0.f};
-  RowOut o{};
-  float k1 = 0.f, k0 = 0.f;
+  float slope = 0.f, k1 = 0.f, k0 = 0.f;
+  const float adv = a.advantages[row], old = a.old_logp[row], ref = a.ref_logp ? a.ref_logp[row] : 0.0f;
   int64_t action = a.actions[row];
   if (used) {
     if (a.grad) load_row<T, 256, kSplitVectors>((const T*)a.logits + row * a.ld + c0, n, threadIdx.x, x);
@@ -516,17 +538,18 @@ __global__ __launch_bounds__(256) void loss_split_gradient_kernel(LossArgs a, Sp
     }
     r.s = lanes_sum<64>(r.s);
     r.t = lanes_sum<64>(r.t);
-    o = row_values(a, r, ws.xa[local], a.advantages[row], a.old_logp[row], a.ref_logp ? a.ref_logp[row] : 0.0f, k1,
-                   k0);
+    slope = row_gradient(a, r, ws.xa[local], adv, old, ref, k1, k0);
   }
   const float factor = (float)(used ? (double)w * inv * (double)a.grad_scale : 0.0);
   if (a.grad)
-    store_gradient<T, 256, kSplitVectors>((T*)a.grad + row * a.ldg + c0, n, threadIdx.x, x, r, o, k1, k0,
+    store_gradient<T, 256, kSplitVectors>((T*)a.grad + row * a.ldg + c0, n, threadIdx.x, x, r, slope, k1, k0,
                                           factor, action - c0, used);
-  if (piece == 0 && threadIdx.x == 0) {
+  if (piece == 0 && threadIdx.x < 64) {
+    const RowOut o = row_values(a, r, used ? ws.xa[local] : 0.0f, adv, old, ref);
+    if (threadIdx.x) return;
     a.logp[row] = used ? o.logp : 0.0f;
     a.entropy[row] = used ? o.entropy : 0.0f;
-    a.values[row] = used ? (double)w * (double)o.value : 0.0;
+    a.values[row] = used ? (double)w * o.value : 0.0;
   }
 }
 
@@ -662,15 +685,15 @@ extern "C" int dz_policy_loss(const dz_policy_loss_args_t* a, dz_stream_t stream
   LossArgs k{};
   k.logits = a->logits; k.ld = a->ld; k.grad = a->dlogits; k.ldg = a->ldg;
   k.actions = a->actions; k.advantages = a->advantages; k.old_logp = a->old_logp;
-  k.ref_logp = a->kl_coef != 0.f ? a->ref_logp : nullptr;   // (0 * inf)
+  k.ref_logp = a->kl_coef != 0.0 ? a->ref_logp : nullptr;   // (0 * inf)
   k.weights = a->weights;
   k.logp = a->logp; k.entropy = a->entropy; k.loss = a->loss; k.status = a->status;
   k.values = sums + kWeightBlocks;
   k.weight_sums = summed && p.form != Form::kOne ? sums : nullptr;
   // 0 in the one-workgroup form means: sum the weights
   k.inv_norm = summed ? 0.0 : 1.0 / (a->normalizer > 0.0 ? a->normalizer : (double)a->rows);
-  k.low = (float)(1.0 - a->clip_low); k.high = (float)(1.0 + a->clip_high);
-  k.kl = a->kl_coef; k.ent = a->entropy_coef; k.grad_scale = a->grad_scale;
+  k.low = 1.0 - a->clip_low; k.high = 1.0 + a->clip_high;
+  k.kl = a->kl_coef; k.ent_coef = a->entropy_coef; k.ent = (float)a->entropy_coef; k.grad_scale = a->grad_scale;
   k.rows = a->rows; k.classes = (int)a->classes;
   if (k.weight_sums) {
     hipLaunchKernelGGL(loss_weights_kernel, dim3(kWeightBlocks), dim3(256), 0, s, a->weights, a->rows, sums);

@@ -888,8 +888,8 @@ typedef struct {
   float* entropy;            /* [rows]                                           */
   uint32_t* status;          /* or NULL                                          */
   void* ws; int64_t ws_bytes;  /* dz_policy_loss_workspace (may be 0); 16-byte aligned, contents arbitrary */
-  double clip_low, clip_high, normalizer;
-  float kl_coef, entropy_coef, grad_scale;
+  double clip_low, clip_high, kl_coef, entropy_coef, normalizer;
+  float grad_scale;
   int32_t reserved2;
 } dz_policy_loss_args_t;
 
