@@ -12,7 +12,8 @@ global norm, master weights, moments in 32 or 8 bits.
     opt.step(bound)
 
 Work is enqueued on the current stream of the parameters' device; nothing synchronises.  A step may
-be captured into a graph: the step count and the learning rate live on the device.
+be captured into a graph: the step count and the learning rate live on the device.  The parameters
+(and bound gradients) have to stay where they are in memory, as for any captured work.
 """
 
 import ctypes
@@ -182,7 +183,7 @@ class AdamW:
         raise ValueError('a gradient shares memory with a parameter')
       last[kind] = max(last[kind], end)
     with _lib.device_guard(self._index):
-      table = torch.zeros(len(grads), dtype=torch.int64, device=self.device)
+      table = _lib.new_output(len(grads), torch.int64, self.device)
       self._upload(grads, table)
     return BoundGradients(self, grads, table, dtype)
 
@@ -236,8 +237,8 @@ class AdamW:
     if self.config.state_bits == 32:
       return self.m.to(dtype), self.v.to(dtype)
     with _lib.device_guard(self._index):
-      m = torch.empty(self.state_size, dtype=dtype, device=self.device)
-      v = torch.empty_like(m)
+      m = _lib.new_output(self.state_size, dtype, self.device)
+      v = _lib.new_output(self.state_size, dtype, self.device)
       _lib.check(self._lib.dz_adamw_moments(
           self.m.data_ptr(), self.v.data_ptr(), self.m_scale.data_ptr(), self.v_scale.data_ptr(),
           self.state_size, code, m.data_ptr(), v.data_ptr(), _lib.stream_ptr(self._index)),

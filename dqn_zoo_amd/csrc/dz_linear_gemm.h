@@ -110,28 +110,32 @@ __device__ __forceinline__ float logistic(float z) {
   else return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
 }
 
+// Infinite z have their limits' values (a factor that vanishes is multiplied by a bounded z; a NaN
+// comes back through the other factor).
+constexpr float kBound = 1e30f;
 template <typename T>
 __device__ __forceinline__ float linear_act(float z, int act) {
   float density;
   switch (act) {
     case DZ_ACT_RELU: return z < 0.f ? 0.f : z;   // (NaN stays)
-    case DZ_ACT_GELU: return __builtin_fmaf(-fabsf(z), normal_tail<T>(z, density), fmaxf(z, 0.f));   // z Phi(z)
-    case DZ_ACT_SILU: return z * logistic<T>(z);
+    case DZ_ACT_GELU: return fmaxf(z, 0.f) - fminf(fabsf(z), kBound) * normal_tail<T>(z, density);   // z Phi(z)
+    case DZ_ACT_SILU: return fmaxf(z, -kBound) * logistic<T>(z);
     default: return z;
   }
 }
 template <typename T>
 __device__ __forceinline__ float linear_act_slope(float z, int act) {
+  const float bounded = fminf(fmaxf(z, -kBound), kBound);
   switch (act) {
     case DZ_ACT_RELU: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
     case DZ_ACT_GELU: {
       float density;
       const float tail = normal_tail<T>(z, density);
-      return __builtin_fmaf(z * 0.39894228040143268f, density, z < 0.f ? tail : 1.0f - tail);
+      return __builtin_fmaf(bounded * 0.39894228040143268f, density, z < 0.f ? tail : 1.0f - tail);
     }
     case DZ_ACT_SILU: {
       const float s = logistic<T>(z);
-      return s * (1.0f + z * (1.0f - s));
+      return s * (1.0f + bounded * (1.0f - s));
     }
     default: return 1.f;
   }

@@ -676,7 +676,7 @@ extern "C" int dz_policy_loss(const dz_policy_loss_args_t* a, dz_stream_t stream
   DZ_REQUIRE(a->logits && a->actions && a->advantages && a->old_logp && a->logp && a->entropy && a->loss);
   DZ_REQUIRE(a->ld >= a->classes && (!a->dlogits || a->ldg >= a->classes));
   DZ_REQUIRE(((uintptr_t)a->ws & 15) == 0);
-  DZ_REQUIRE(a->clip_low >= 0.0 && a->clip_high >= 0.0 && a->normalizer >= 0.0);
+  DZ_REQUIRE(a->clip_low >= 0.0 && a->clip_high >= 0.0 && a->normalizer >= 0.0 && a->normalizer < __builtin_inf());
   const Plan p = make_plan(a->dtype, a->rows, (int)a->classes);
   DZ_REQUIRE(p.ws_bytes == 0 || (a->ws && a->ws_bytes >= p.ws_bytes));
   const hipStream_t s = dz_s(stream);

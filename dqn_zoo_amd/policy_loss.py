@@ -71,6 +71,23 @@ def _matrix(name, t, shape, dtype, device):
   return max(ld, cols)
 
 
+def _check_apart(out, **inputs):
+  """A row's outputs may be written while another workgroup still reads that row's inputs."""
+  def extent(t):
+    last = sum((s - 1) * d for s, d in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + t.element_size() * (last + 1)
+  outs = [(n, t) for n, t in zip(out._fields, out) if t is not None]
+  for i, (name, t) in enumerate(outs):
+    a, b = extent(t)
+    others = outs[:i] + [(n, x) for n, x in inputs.items() if x is not None]
+    for other, x in others:
+      if other == 'logits' and name == 'dlogits' and x.data_ptr() == a and x.stride() == t.stride():
+        continue
+      c, d = extent(x)
+      if a < d and c < b:
+        raise ValueError('out.%s overlaps %s' % (name, other))
+
+
 def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.Tensor,
                 old_logp: torch.Tensor, ref_logp: typing.Optional[torch.Tensor] = None,
                 weights: typing.Optional[torch.Tensor] = None, *,
@@ -127,26 +144,24 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.T
   with _lib.device_guard(device):
     if out is None:
       where = logits.device
-      out = PolicyLossOutputs(
-          _lib.new_output((), f32, where), _lib.new_output(rows, f32, where),
-          _lib.new_output(rows, f32, where),
-          _lib.new_output(shape, logits.dtype, where) if with_gradient else None)
+      logp, entropy = _lib.new_output((2, rows), f32, where).unbind()
+      out = PolicyLossOutputs(_lib.new_output((), f32, where), logp, entropy,
+                              _lib.new_output(shape, logits.dtype, where) if with_gradient else None)
     else:
       if _row_vector('out.loss', out.loss.view(1), 1, f32, device) is None or (
           out.dlogits is None) == with_gradient:
         raise ValueError('out.dlogits must be given exactly if with_gradient')
       _row_vector('out.logp', out.logp, rows, f32, device)
       _row_vector('out.entropy', out.entropy, rows, f32, device)
+      if with_gradient:
+        _matrix('out.dlogits', out.dlogits, shape, logits.dtype, device)
+      _check_apart(out, logits=logits, actions=actions, advantages=advantages, old_logp=old_logp,
+                   ref_logp=ref_logp, weights=weights, status=status)
     a.loss, a.logp, a.entropy = out.loss.data_ptr(), out.logp.data_ptr(), out.entropy.data_ptr()
     if with_gradient:
       g = out.dlogits
       a.ldg = _matrix('out.dlogits', g, shape, logits.dtype, device)
       a.dlogits = g.data_ptr()
-      if a.dlogits != a.logits or a.ldg != a.ld:
-        size = logits.element_size()
-        if (a.dlogits < a.logits + ((rows - 1) * a.ld + classes) * size and
-            a.logits < a.dlogits + ((rows - 1) * a.ldg + classes) * size):
-          raise ValueError('out.dlogits overlaps the logits without being them')
     lib = _lib.load()
     need = ctypes.c_int64()
     _lib.check(lib.dz_policy_loss_workspace(code, rows, classes, ctypes.byref(need)),

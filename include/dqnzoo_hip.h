@@ -778,7 +778,8 @@ int dz_atari_observation(const uint8_t* const* frames, int n_frames, int height,
  * scale per DZ_ADAMW_STATE_BLOCK elements; m as OCP e4m3, v as an unsigned float
  * of 5 exponent and 3 fraction bits (code c >= 8: (1 + (c & 7)/8) 2^((c >> 3) - 31),
  * c < 8: c 2^-33), both rounded at random (counter-based, keyed by seed and step).
- * A gradient that is not finite makes the parameters it meets NaN.              */
+ * A gradient that is not finite makes the parameters it meets NaN (8-bit moments: the
+ * rest of its block with the next step), a norm that is NaN every parameter.        */
 #define DZ_ADAMW_STATE_BLOCK 256
 #define DZ_ADAMW_CHUNK 4096
 typedef struct {
@@ -868,7 +869,7 @@ int dz_linear_backward(const dz_linear_args_t* args, dz_stream_t stream);
  *   loss = sum_i weights[i] value[i] / norm
  * norm: `normalizer`, or the sum of the weights (the number of rows without weights) where
  * that is 0.  dlogits = grad_scale * d loss / d logits, rounded once; it may be the logits'
- * own buffer (same pointer and pitch).  A row of weight 0 is not looked at (its action may
+ * own buffer (same pointer and pitch); no other output may lie on an input.  A row of weight 0 is not looked at (its action may
  * be anything): logp, entropy and gradient 0.  An action outside [0, classes) makes its row
  * and the loss NaN and sets DZ_ST_BAD_INDEX in `status`.  A row whose logits are all -inf,
  * or hold NaN or +inf, is NaN.  All weights 0: loss and gradient 0.                      */

@@ -227,6 +227,26 @@ def test_special_values_stay_in_their_rows_and_columns():
   assert (y[9][torch.isfinite(y[9])] == 0).all()       # relu(-inf)
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+def test_activations_far_out(dtype):
+  """Infinite and very large pre-activations have the limits' values and slopes, NaN stays NaN."""
+  from dqn_zoo_amd import linear
+  inf = float('inf')
+  far = torch.tensor([inf, -inf, 6e4, -6e4, 40.0, -40.0, 0.0, float('nan')], dtype=dtype, device='cuda')
+  x, w = torch.ones(1, 1, dtype=dtype, device='cuda'), torch.zeros(1, 8, dtype=dtype, device='cuda')
+  for name in ('relu', 'gelu', 'silu'):
+    y, z = linear.linear(x, w, far, activation=name, save_preact=True)
+    assert torch.equal(z[0, :7], far[:7]) and torch.isnan(z[0, 7])
+    want = torch.tensor([inf, 0, 6e4, 0, 40, 0, 0], dtype=dtype, device='cuda')
+    # (silu(-40) is -1.7e-16)
+    assert torch.allclose(y[0, :7].float(), want.float(), atol=1e-15, rtol=0) and torch.isnan(y[0, 7]), (name, y)
+    dy = torch.ones(1, 8, dtype=dtype, device='cuda')
+    _, _, db = linear.linear_backward(dy, x, w, activation=name, preact=z, need=(False, False, True))
+    zero = 0.0 if name == 'relu' else 0.5
+    want = torch.tensor([1, 0, 1, 0, 1, 0, zero], dtype=dtype, device='cuda')
+    assert torch.allclose(db[:7].float(), want.float(), atol=1e-14, rtol=2 * U32) and torch.isnan(db[7]), (name, db)
+
+
 @pytest.mark.parametrize('m,k,n', [(1, 3136, 512), (300, 264, 520), (8, 4096, 64)])
 def test_captured_and_replayed(m, k, n):
   from dqn_zoo_amd import _lib, linear

@@ -352,6 +352,11 @@ def test_refusals():
   refused(ValueError, 'exactly if', out=o._replace(dlogits=None))
   buf = torch.zeros(5, 6, device='cuda')
   refused(ValueError, 'overlaps', logits=buf[:4], out=o._replace(dlogits=buf[1:]))
+  for name in ('advantages', 'old_logp', 'ref_logp'):   # another workgroup may still read them
+    refused(ValueError, 'out.logp overlaps ' + name, out=o._replace(logp=i[name]))
+  w = torch.ones(4, device='cuda')
+  refused(ValueError, 'out.entropy overlaps weights', weights=w, out=o._replace(entropy=w))
+  refused(ValueError, 'out.entropy overlaps logp', out=o._replace(entropy=o.logp))
   # the C entry refuses before it launches anything
   lib = _lib.load()
   n = ctypes.c_int64()
