@@ -23,4 +23,5 @@ const DzLinearLaunch* dz_linear_launch_f16();
 
 constexpr DzGemmShape kGemmTiles[] = {{64, 64, 2, 2, 3}, {128, 128, 2, 2, 2}, {256, 256, 2, 4, 2}};
 constexpr int kGemmTileCount = sizeof(kGemmTiles) / sizeof(kGemmTiles[0]);
-constexpr int kRowsTile = -1;   // linear_rows_kernel: up to kRowsM rows
+constexpr int kRowsTile = -1;   // linear_rows_kernel
+constexpr int kRowsMost = 32;   // its rows

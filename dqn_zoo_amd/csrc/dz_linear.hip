@@ -44,9 +44,9 @@ DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool a_kc, b
   const int bk = (int)(128 / elem);
   const int64_t stages = (k + bk - 1) / bk;
   const double bytes = (double)(m + n) * k * elem;
-  if (a_kc && m <= kRowsM) {
+  if (a_kc && m <= kRowsMost) {
     const int64_t rounds = ((n + kRowsN - 1) / kRowsN + kCus - 1) / kCus, depth = (stages + kRowsWaves - 1) / kRowsWaves;
-    const double work = rounds * depth * (elem == 2 ? 0.30 : 0.56), flow = bytes / (b_kc || elem == 4 ? 5.3e6 : 2.4e6);
+    const double work = rounds * depth * (elem == 2 ? 0.30 : m <= 16 ? 0.56 : 1.0), flow = bytes / (b_kc || elem == 4 ? 5.3e6 : 2.4e6);
     best_us = 3.0 + (work > flow ? work : flow) + 0.9 * (rounds - 1);
     best.tile = kRowsTile;
     best.splits = 1;

@@ -449,18 +449,20 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_gemm_kernel(DzGemmArgs p)
   }
 }
 
-// Up to 16 rows (the tokens of a generation step, one observation): a workgroup has 32 columns and
+// Up to 16 or 32 rows (the tokens of a generation step, one observation, a learner's batch of 32): a
+// workgroup has 32 columns and
 // the whole depth, its eight waves take its stages in turn, each through a ring of its own -- no barrier
 // until the waves' sums meet in LDS, no slabs, one launch.  Bound by the weight's bytes: 64 KB of them
 // are on their way in each CU.
-constexpr int kRowsWaves = 8, kRowsBuffers = 3, kRowsM = 16, kRowsN = 32;
-template <typename T, bool B_KC>
+constexpr int kRowsWaves = 8, kRowsN = 32;
+constexpr int rows_buffers(int rows) { return rows == 16 ? 3 : 2; }   // (160 KB of LDS)
+template <typename T, bool B_KC, int ROWS>
 __global__ __launch_bounds__(64 * kRowsWaves) void linear_rows_kernel(DzGemmArgs p) {
-  constexpr int BK = 128 / sizeof(T), FN = kRowsN / 16;
-  constexpr int A_BYTES = kRowsM * 128, STAGE = (kRowsM + kRowsN) * 128, RING = kRowsBuffers * STAGE;
-  using SA = Stager<T, true, kRowsM, 64>;
+  constexpr int BK = 128 / sizeof(T), FM = ROWS / 16, FN = kRowsN / 16, NBUF = rows_buffers(ROWS);
+  constexpr int A_BYTES = ROWS * 128, STAGE = (ROWS + kRowsN) * 128, RING = NBUF * STAGE;
+  using SA = Stager<T, true, ROWS, 64>;
   using SB = Stager<T, B_KC, kRowsN, 64>;
-  constexpr int OUT = (kRowsBuffers - 2) * (SA::PER + SB::PER);
+  constexpr int OUT = (NBUF - 2) * (SA::PER + SB::PER);
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j0 = blockIdx.x * kRowsN;
@@ -471,7 +473,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear_rows_kernel(DzGemmArgs
   char* ring = lds + wave * RING;
   const unsigned lds0 = (unsigned)(uintptr_t)ring;
 
-  f32x4 acc[FN] = {};
+  f32x4 acc[FM][FN] = {};
   SA ra;
   SB rb;
   ra.init((const T*)p.a, p.lda, 0, p.m, 0, 0, lane);
@@ -494,13 +496,13 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear_rows_kernel(DzGemmArgs
     }
   };
 #pragma unroll
-  for (int n = 0; n < kRowsBuffers - 1; ++n)
+  for (int n = 0; n < NBUF - 1; ++n)
     if (n < stages) fetch(n, n);
   auto step = [&](int t, int buf) {
     // the next buffer's reads are done (their products are issued), stage t is here
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (t + kRowsBuffers - 1 < stages) {
-      fetch(t + kRowsBuffers - 1, (buf + kRowsBuffers - 1) % kRowsBuffers);
+    if (t + NBUF - 1 < stages) {
+      fetch(t + NBUF - 1, (buf + NBUF - 1) % NBUF);
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OUT + SA::PER + SB::PER) : "memory");
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -513,35 +515,42 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear_rows_kernel(DzGemmArgs
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const auto fa = Operand<T, true, kRowsM>::fragment(sa, 0, s, lane);
+      typename MfmaFrag<T>::V fa[FM];
 #pragma unroll
-      for (int f = 0; f < FN; ++f)
-        acc[f] = mfma16(Operand<T, B_KC, kRowsN>::fragment(sa + A_BYTES, f, s, lane), fa, acc[f]);
+      for (int i = 0; i < FM; ++i) fa[i] = Operand<T, true, ROWS>::fragment(sa, i, s, lane);
+#pragma unroll
+      for (int f = 0; f < FN; ++f) {
+        const auto fb = Operand<T, B_KC, kRowsN>::fragment(sa + A_BYTES, f, s, lane);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) acc[i][f] = mfma16(fb, fa[i], acc[i][f]);
+      }
     }
   };
   int t = 0;
-  for (; t + kRowsBuffers <= stages; t += kRowsBuffers) {
+  for (; t + NBUF <= stages; t += NBUF) {
 #pragma unroll
-    for (int n = 0; n < kRowsBuffers; ++n) step(t + n, n);
+    for (int n = 0; n < NBUF; ++n) step(t + n, n);
   }
 #pragma unroll
-  for (int n = 0; n < kRowsBuffers - 1; ++n)
+  for (int n = 0; n < NBUF - 1; ++n)
     if (t + n < stages) step(t + n, n);
 
   __syncthreads();
   float* sums = (float*)lds;   // [wave][row][column]
 #pragma unroll
-  for (int f = 0; f < FN; ++f)
-    *(f32x4*)(sums + (wave * kRowsM + (lane & 15)) * kRowsN + f * 16 + 4 * (lane >> 4)) = acc[f];
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int f = 0; f < FN; ++f)
+      *(f32x4*)(sums + (wave * ROWS + i * 16 + (lane & 15)) * kRowsN + f * 16 + 4 * (lane >> 4)) = acc[i][f];
   __syncthreads();
-  static_assert(kRowsWaves * 64 >= kRowsM * kRowsN / 4, "a thread per four columns");
+  static_assert(kRowsWaves * 64 >= ROWS * kRowsN / 4, "a thread per four columns");
   const int row = threadIdx.x / (kRowsN / 4), c = threadIdx.x % (kRowsN / 4) * 4;
-  if (row >= p.m || row >= kRowsM || j0 + c >= p.n) return;
+  if (row >= p.m || row >= ROWS || j0 + c >= p.n) return;
   Epilogue<T, 4> epi;
   epi.init(p, j0 + c);
   f32x4 v = *(const f32x4*)(sums + row * kRowsN + c);
 #pragma unroll
-  for (int w = 1; w < kRowsWaves; ++w) v += *(const f32x4*)(sums + (w * kRowsM + row) * kRowsN + c);
+  for (int w = 1; w < kRowsWaves; ++w) v += *(const f32x4*)(sums + (w * ROWS + row) * kRowsN + c);
   const float d[4] = {v[0], v[1], v[2], v[3]};
   epi.row(p, row, j0 + c, d);
 }
