@@ -5,7 +5,7 @@
 #include "dz_linear_gemm.h"
 
 struct DzGemmPlan {
-  int tile;            // index of the tile sizes, or kRowsTile
+  int tile;            // index of the tile sizes, or kRows*Tile
   int splits, k_split;
   int64_t slab_bytes;  // 0 without splits
 };
@@ -23,5 +23,6 @@ const DzLinearLaunch* dz_linear_launch_f16();
 
 constexpr DzGemmShape kGemmTiles[] = {{64, 64, 2, 2, 3}, {128, 128, 2, 2, 2}, {256, 256, 2, 4, 2}};
 constexpr int kGemmTileCount = sizeof(kGemmTiles) / sizeof(kGemmTiles[0]);
-constexpr int kRowsTile = -1;   // linear_rows_kernel
-constexpr int kRowsMost = 32;   // its rows
+constexpr int kRowsTile = -1;      // linear_rows_kernel
+constexpr int kRowsAnyTile = -2;   // linear_rows_any_kernel: operands of any alignment
+constexpr int kRowsMost = 32;      // their rows

@@ -30,6 +30,7 @@ int64_t packed_bytes(const Matrix& x, int64_t elem) { return round_up(x.rows * p
 // takes when its CU has nothing else (`alone`, of one workgroup on the chip, up to `full` of 256),
 // and what each of many costs a busy CU.
 struct TileCost { double alone, full, busy; int per_cu; };
+constexpr double kAnySlower = 1.5;   // the rows' kernel through registers
 constexpr TileCost kCost16[] = {{0.22, 0.25, 0.185, 3}, {0.61, 0.95, 0.53, 2}, {1.10, 1.90, 1.90, 1}};
 constexpr TileCost kCost32[] = {{0.58, 0.60, 0.455, 3}, {2.00, 2.00, 1.85, 2}, {7.20, 7.40, 7.40, 1}};
 
@@ -38,17 +39,19 @@ constexpr TileCost kCost32[] = {{0.58, 0.60, 0.455, 3}, {2.00, 2.00, 1.85, 2}, {
 // rows' kernel: 1 x 3136 x 512 in 5.2 us against 8.7 (tile 64 x 64, 7 splits), 16 x 8192 x 4096 from
 // a transposed weight in 15.0 against 15.7; its 64-byte pieces of an (in, out) weight's rows come at
 // 2.4 TB/s (16 x 8192 x 4096: 25.8 against 16.8).
-DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool a_kc, bool b_kc) {
+DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool a_kc, bool b_kc, int64_t copied = 0,
+                     bool rows = true) {
   DzGemmPlan best{};
   double best_us = 1e30;
   const int bk = (int)(128 / elem);
   const int64_t stages = (k + bk - 1) / bk;
   const double bytes = (double)(m + n) * k * elem;
-  if (a_kc && m <= kRowsMost) {
+  const double copy = copied ? 3.0 + 2.0 * copied / 4e6 : 0.0;   // `copied` bytes of operands, a launch of their own
+  if (rows && a_kc && m <= kRowsMost) {
     const int64_t rounds = ((n + kRowsN - 1) / kRowsN + kCus - 1) / kCus, depth = (stages + kRowsWaves - 1) / kRowsWaves;
     const double work = rounds * depth * (elem == 2 ? 0.30 : m <= 16 ? 0.56 : 1.0), flow = bytes / (b_kc || elem == 4 ? 5.3e6 : 2.4e6);
-    best_us = 3.0 + (work > flow ? work : flow) + 0.9 * (rounds - 1);
-    best.tile = kRowsTile;
+    best_us = 3.0 + (work > flow ? work : flow) * (copied ? kAnySlower : 1.0) + 0.9 * (rounds - 1);
+    best.tile = copied ? kRowsAnyTile : kRowsTile;
     best.splits = 1;
     best.k_split = (int)(stages * bk);
   }
@@ -63,7 +66,7 @@ DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool a_kc, b
       const double load = groups < kCus ? (double)groups / kCus : 1.0;
       const double one = c.alone + (c.full - c.alone) * load;
       const double stage = rounds * one > per_cu * c.busy ? rounds * one : per_cu * c.busy;
-      double us = 3.5 + (depth * stage > bytes / 5.3e6 ? depth * stage : bytes / 5.3e6);
+      double us = 3.5 + copy + (depth * stage > bytes / 5.3e6 ? depth * stage : bytes / 5.3e6);
       if (s > 1) us += 2.8 + 0.1 * s + 2.0 * s * (double)m * n * 4 / 3e6;
       if (us < best_us) {
         best_us = us;
@@ -105,7 +108,10 @@ Layout plan_forward(const dz_linear_args_t* a) {
   const int64_t elem = dz_elem_bytes(a->dtype);
   l.pack_x = !readable(x_of(a), elem);
   l.pack_w = !readable(w_of(a), elem);
-  l.fwd = plan_gemm(a->m, a->n, a->k, elem, true, a->w_transposed != 0);
+  const int64_t copied = (l.pack_x ? packed_bytes(x_of(a), elem) : 0) + (l.pack_w ? packed_bytes(w_of(a), elem) : 0);
+  // (sizes alone: the copies and the slabs that a call may need, so not the rows' kernel)
+  l.fwd = plan_gemm(a->m, a->n, a->k, elem, true, a->w_transposed != 0, copied, a->x && a->w);
+  if (l.fwd.tile == kRowsAnyTile) l.pack_x = l.pack_w = false;
   if (l.pack_x) { l.x_at = l.bytes; l.bytes += packed_bytes(x_of(a), elem); }
   if (l.pack_w) { l.w_at = l.bytes; l.bytes += packed_bytes(w_of(a), elem); }
   l.slabs_at = l.bytes;
@@ -121,7 +127,9 @@ Layout plan_backward(const dz_linear_args_t* a) {
   l.form_dz = (dx || dw) && (a->activation != DZ_ACT_NONE || !readable(dy, elem));
   l.pack_x = dw && !readable(x_of(a), elem);
   l.pack_w = dx && !readable(w_of(a), elem);
-  if (dx) l.dx = plan_gemm(a->m, a->k, a->n, elem, true, a->w_transposed == 0);
+  if (dx) l.dx = plan_gemm(a->m, a->k, a->n, elem, true, a->w_transposed == 0,
+                           l.pack_w ? packed_bytes(w_of(a), elem) : 0, !sizes_only);
+  if (l.dx.tile == kRowsAnyTile) l.pack_w = false;
   if (dw) l.dw = a->w_transposed ? plan_gemm(a->n, a->k, a->m, elem, false, false)
                                        : plan_gemm(a->k, a->n, a->m, elem, false, false);
   // rows of one chunk of the column sums: four workgroups per CU, if the rows allow

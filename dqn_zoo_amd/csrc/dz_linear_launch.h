@@ -33,25 +33,26 @@ int launch_gemm_kind(const DzGemmArgs& p, const DzGemmPlan& plan, hipStream_t s)
 }
 
 template <typename T, bool B_KC, int ROWS>
-int launch_rows_of(const DzGemmArgs& p, hipStream_t s) {
-  constexpr int kLds = kRowsWaves * rows_buffers(ROWS) * (ROWS + kRowsN) * 128;
-  auto kernel = linear_rows_kernel<T, B_KC, ROWS>;
-  DZ_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-  hipLaunchKernelGGL(kernel, dim3((p.n + kRowsN - 1) / kRowsN), dim3(64 * kRowsWaves), kLds, s, p);
+int launch_rows_of(const DzGemmArgs& p, bool any, hipStream_t s) {
+  const int lds = kRowsWaves * (any ? 2 : rows_buffers(ROWS)) * (ROWS + kRowsN) * 128;
+  auto kernel = any ? linear_rows_any_kernel<T, B_KC, ROWS> : linear_rows_kernel<T, B_KC, ROWS>;
+  DZ_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  hipLaunchKernelGGL(kernel, dim3((p.n + kRowsN - 1) / kRowsN), dim3(64 * kRowsWaves), lds, s, p);
   DZ_LAUNCH_CHECK();
   return DZ_OK;
 }
 
 template <typename T, bool B_KC>
-int launch_rows(const DzGemmArgs& p, hipStream_t s) {
-  return p.m <= 16 ? launch_rows_of<T, B_KC, 16>(p, s) : launch_rows_of<T, B_KC, 32>(p, s);
+int launch_rows(const DzGemmArgs& p, bool any, hipStream_t s) {
+  return p.m <= 16 ? launch_rows_of<T, B_KC, 16>(p, any, s) : launch_rows_of<T, B_KC, 32>(p, any, s);
 }
 
 template <typename T>
 int launch_gemm(const DzGemmArgs& p, const DzGemmPlan& plan, bool a_kc, bool b_kc, hipStream_t s) {
-  if (plan.tile == kRowsTile) {
+  if (plan.tile < 0) {
     if (!a_kc || p.m > kRowsMost || p.splits != 1) return DZ_ERR_UNSUPPORTED;
-    return b_kc ? launch_rows<T, true>(p, s) : launch_rows<T, false>(p, s);
+    const bool any = plan.tile == kRowsAnyTile;
+    return b_kc ? launch_rows<T, true>(p, any, s) : launch_rows<T, false>(p, any, s);
   }
   int rc;
   if (a_kc && b_kc) rc = launch_gemm_kind<T, true, true>(p, plan, s);

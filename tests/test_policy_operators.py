@@ -132,9 +132,10 @@ def test_c_entries_refuse(lib):
     assert lib.dz_linear_backward(ctypes.byref(a), None) == bad
   ok = dict(x=4096, ldx=8, w=4096, ldw=8, y=4096, ldy=8)
   for change in (dict(x=None), dict(w=None), dict(y=None), dict(ldx=7), dict(ldw=7), dict(ldy=7),
-                 dict(residual=4096, ldr=7), dict(preact=4096, ldz=7),
-                 dict(x=4098)):   # its copy needs a workspace
+                 dict(residual=4096, ldr=7), dict(preact=4096, ldz=7)):
     assert lib.dz_linear(ctypes.byref(_linear_args(8, 8, 8, **{**ok, **change})), None) == bad, change
+  # (above 32 rows an operand that cannot be read where it lies needs a workspace for its copy)
+  assert lib.dz_linear(ctypes.byref(_linear_args(64, 8, 8, **{**ok, 'x': 4098})), None) == bad
   back = dict(x=4096, ldx=8, w=4096, ldw=8, dy=4096, lddy=8, dx=4096, lddx=8, dw=4096, lddw=8)
   for change in (dict(dy=None), dict(lddy=7), dict(lddx=7), dict(lddw=7), dict(activation=1), dict(x=None),
                  dict(w=None), dict(dx=None, dw=None)):
