@@ -35,7 +35,7 @@ constexpr TileCost kCost16[] = {{0.22, 0.25, 0.185, 3}, {0.61, 0.95, 0.53, 2}, {
 constexpr TileCost kCost32[] = {{0.58, 0.60, 0.455, 3}, {2.00, 2.00, 1.85, 2}, {7.20, 7.40, 7.40, 1}};
 
 // Tile and number of splits: the least estimated time, with the operands' bytes at 5.3 TB/s as its
-// floor.  A split costs its slab's way out and back and a second launch.  Up to 16 rows may take the
+// floor.  A split costs its slab's way out and back and a second launch.  Up to 32 rows may take the
 // rows' kernel: 1 x 3136 x 512 in 5.2 us against 8.7 (tile 64 x 64, 7 splits), 16 x 8192 x 4096 from
 // a transposed weight in 15.0 against 15.7; its 64-byte pieces of an (in, out) weight's rows come at
 // 2.4 TB/s (16 x 8192 x 4096: 25.8 against 16.8).

@@ -16,8 +16,9 @@
 //
 // Both operands come by 16-byte LDS-DMA: their rows begin at multiples of 16 bytes and hold whole
 // 16-byte units (operands that do not are copied into such rows first, linear_pack_kernel, zeros
-// behind their ends; up to 32 rows of A come through registers instead, linear_rows_any_kernel).  What is past an edge along the output index is read from a clamped place and
-// not stored; what is past it along k is zeroed in LDS.
+// behind their ends; with up to 32 rows of A both come through registers instead,
+// linear_rows_any_kernel).  What is past an edge along the output index is read from a clamped place
+// and not stored; what is past it along k is zeroed in LDS.
 //
 // MFMA 16 x 16 with the operands exchanged (rows of the instruction are columns of D): a lane ends
 // with four adjacent columns of one row, so that bias, residual and outputs are vector accesses.

@@ -857,7 +857,8 @@ typedef struct {
 /* Bytes of workspace for the call that these arguments make (backward: 0 dz_linear, 1
  * dz_linear_backward); may be 0.  Without pointers (x, w, dy NULL): enough for every call
  * of these dtype, activation, sizes and w_transposed.  Operands whose rows are not whole
- * 16-byte units at 16-byte addresses are copied into such rows there.              */
+ * 16-byte units at 16-byte addresses are copied into such rows there (32 rows of x and
+ * fewer are mostly multiplied where they lie, without a workspace).                */
 int dz_linear_workspace(const dz_linear_args_t* args, int backward, int64_t* bytes);
 int dz_linear(const dz_linear_args_t* args, dz_stream_t stream);
 int dz_linear_backward(const dz_linear_args_t* args, dz_stream_t stream);

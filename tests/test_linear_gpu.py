@@ -99,6 +99,20 @@ def test_backward(m, k, n, dtype, transposed):
     assert got[1].stride() == ((1, k) if transposed and n > 1 and k > 1 else got[1].stride())
 
 
+@pytest.mark.parametrize('m,k,n', [(9, 1951, 2057), (1, 513, 3137), (32, 3001, 1001), (31, 1001, 257), (33, 1001, 257)])
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('transposed', [False, True])
+def test_few_rows_of_any_alignment(m, k, n, dtype, transposed):
+  from dqn_zoo_amd import linear
+  for pad in (1, 3, 8):
+    x, w, b, r = _make(m, k, n, dtype, m + k + n, transposed, pad)
+    y, z = linear.linear(x, w, b, activation='silu', residual=r, save_preact=True)
+    _check_forward(x, w, b, r, 'silu', y, z, dtype)
+    dy = _pitched(torch.randn(m, n, generator=torch.Generator().manual_seed(3)).to(dtype).cuda(), pad)
+    got = linear.linear_backward(dy, x, w, activation='silu', preact=z)
+    _check_backward(dy, x, w, 'silu', z, got, dtype)
+
+
 def _check_backward(dy, x, w, activation, preact, got, dtype, kind=None):
   kind = kind or dtype
   dyn, xn, wn, zn = _np(dy), _np(x), _np(w), _np(preact)
