@@ -7,6 +7,7 @@ namespace {
 
 constexpr int kCus = 256;
 constexpr int64_t kMaxPitchBytes = 1 << 24;   // 256 rows of it in a 32-bit offset
+constexpr int64_t kMaxThreads = 1ll << 32;    // of one launch, along one axis of its grid
 
 const DzLinearLaunch* launches(int dtype) {
   return dtype == DZ_F32 ? dz_linear_launch_f32() : dtype == DZ_BF16 ? dz_linear_launch_bf16()
@@ -59,6 +60,7 @@ DzGemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, int64_t elem, bool a_kc, b
     const DzGemmShape g = kGemmTiles[t];
     const TileCost c = elem == 2 ? kCost16[t] : kCost32[t];
     const int64_t tiles = ((m + g.bm - 1) / g.bm) * ((n + g.bn - 1) / g.bn);
+    if (t + 1 < kGemmTileCount && tiles * g.wm * g.wn * 64 >= kMaxThreads) continue;
     for (int s = 1; s <= kMaxSplits; s *= 2) {
       if (s > 1 && (stages / s < 2 || tiles * s > 4 * kCus)) break;
       const int64_t depth = (stages + s - 1) / s, groups = tiles * s;

@@ -13,7 +13,7 @@ int launch_gemm_tile(const DzGemmArgs& p, hipStream_t s) {
   constexpr int wm = A_KC && B_KC && t.wm != t.wn ? t.wn : t.wm, wn = A_KC && B_KC && t.wm != t.wn ? t.wm : t.wn;
   constexpr int kLds = t.buffers * (t.bm + t.bn) * 128;
   const int64_t tiles = (int64_t)((p.m + t.bm - 1) / t.bm) * ((p.n + t.bn - 1) / t.bn);
-  if (tiles >= (1ll << 31)) return DZ_ERR_UNSUPPORTED;
+  if (tiles * 64 * t.wm * t.wn >= (1ll << 32)) return DZ_ERR_UNSUPPORTED;
   auto kernel = linear_gemm_kernel<T, A_KC, B_KC, t.bm, t.bn, wm, wn, t.buffers>;
   if (kLds > 65536)
     DZ_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));

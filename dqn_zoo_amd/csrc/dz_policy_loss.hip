@@ -566,6 +566,7 @@ struct Plan {
 };
 
 constexpr int64_t kCacheBytes = 128ll << 20;
+constexpr int64_t kMostGroups = 1 << 20, kMaxThreads = 1ll << 32;   // a launch has fewer than kMaxThreads threads
 
 Plan make_plan(int dtype, int64_t rows, int classes) {
   Plan p{};
@@ -576,6 +577,7 @@ Plan make_plan(int dtype, int64_t rows, int classes) {
     while (p.lanes * 8 < classes) p.lanes *= 2;
     const int64_t per = 256 / p.lanes;
     p.blocks = (rows + per - 1) / per;
+    if (p.blocks > kMostGroups) p.blocks = kMostGroups;   // (which go round)
     p.form = p.blocks <= 2 ? Form::kOne : Form::kFew;
     p.ws_bytes = p.form == Form::kOne ? 0 : bytes + p.blocks * 8;
     return p;
@@ -678,6 +680,7 @@ extern "C" int dz_policy_loss(const dz_policy_loss_args_t* a, dz_stream_t stream
   DZ_REQUIRE(((uintptr_t)a->ws & 15) == 0);
   DZ_REQUIRE(a->clip_low >= 0.0 && a->clip_high >= 0.0 && a->normalizer >= 0.0 && a->normalizer < __builtin_inf());
   const Plan p = make_plan(a->dtype, a->rows, (int)a->classes);
+  DZ_REQUIRE(p.form != Form::kTeam || p.blocks * (p.team < 256 ? 256 : p.team) < kMaxThreads);
   DZ_REQUIRE(p.ws_bytes == 0 || (a->ws && a->ws_bytes >= p.ws_bytes));
   const hipStream_t s = dz_s(stream);
   double* sums = (double*)a->ws;

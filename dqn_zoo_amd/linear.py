@@ -9,7 +9,8 @@ else: any sizes from one row on, float32, bfloat16 or float16, strided rows, the
     y, z = linear.linear(x, w, b, activation='gelu', save_preact=True)
     dx, dw, db = linear.linear_backward(dy, x, w, activation='gelu', preact=z)
 
-Work is enqueued on the current stream of the tensors' device; nothing synchronises.
+Plain buffers in and out, no autograd.  Work is enqueued on the current stream of the tensors'
+device; nothing synchronises.
 """
 
 import ctypes

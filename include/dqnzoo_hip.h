@@ -870,14 +870,17 @@ int dz_linear_backward(const dz_linear_args_t* args, dz_stream_t stream);
  *   loss = sum_i weights[i] value[i] / norm
  * norm: `normalizer`, or the sum of the weights (the number of rows without weights) where
  * that is 0.  dlogits = grad_scale * d loss / d logits, rounded once; it may be the logits'
- * own buffer (same pointer and pitch); no other output may lie on an input.  A row of weight 0 is not looked at (its action may
- * be anything): logp, entropy and gradient 0.  An action outside [0, classes) makes its row
- * and the loss NaN and sets DZ_ST_BAD_INDEX in `status`.  A row whose logits are all -inf,
- * or hold NaN or +inf, is NaN.  All weights 0: loss and gradient 0.                      */
+ * own buffer (same pointer and pitch); no other output may lie on an input.  A row of
+ * weight 0 is not looked at (its action may be anything): logp, entropy and gradient 0.  An
+ * action outside [0, classes) makes its row and the loss NaN and sets DZ_ST_BAD_INDEX in
+ * `status`.  A row whose logits are all -inf, or hold NaN or +inf, is NaN.  All weights 0:
+ * loss and gradient 0.                                                                   */
 typedef struct {
   int32_t dtype;             /* of logits and dlogits                            */
   int32_t reserved;
-  int64_t rows, classes;     /* classes < 2^30, rows < 2^31                      */
+  int64_t rows, classes;     /* classes < 2^30, rows < 2^31; a launch has fewer than 2^32
+                              * threads: above 256 classes rows < 2^26, 2^24 or 2^22, as a
+                              * row takes 64, 256 or 1024 of them                 */
   const void* logits; int64_t ld;
   const int64_t* actions;    /* [rows]                                           */
   const float* advantages;

@@ -133,6 +133,15 @@ def _check_backward(dy, x, w, activation, preact, got, dtype, kind=None):
     _close(_np(db), want[2], _sum_tol(xn.shape[0], mag.sum(0)) + (slope + 0 * dz).sum(0), kind, 'db')
 
 
+def test_more_rows_than_a_launch_of_small_tiles_has():
+  from dqn_zoo_amd import linear
+  m = (1 << 30) + 77   # 2^24 tiles of 64 rows and 256 threads
+  x = torch.arange(-128, 128, device='cuda').to(BF16).repeat(m // 256 + 1)[:m].view(m, 1)
+  w = torch.full((1, 1), -2.0, dtype=BF16, device='cuda')
+  y = linear.linear(x, w)
+  assert torch.equal(y, x.mul_(-2))   # exact: at most 9 bits
+
+
 # every tile, whole and ragged, with and without splits along the depth
 @pytest.mark.parametrize('m,k,n', [(512, 512, 512), (520, 1096, 776), (1024, 64, 2048), (2048, 2048, 2048),
                                    (8, 8192, 256), (4096, 24, 264), (300, 4104, 136), (16, 40, 20000),

@@ -300,6 +300,25 @@ def test_captured_and_replayed(rows, classes):
   _lib.load().dz_graph_destroy(own)
 
 
+def test_more_rows_than_workgroups():
+  # (2^20 workgroups of 8 rows go round; the halves do not)
+  from dqn_zoo_amd import policy_loss as pl
+  rows, classes = (1 << 23) + 1003, 130
+  g = torch.Generator('cuda').manual_seed(11)
+  logits = torch.randn(4099, classes, generator=g, device='cuda').bfloat16().repeat(rows // 4099 + 1, 1)[:rows]
+  actions = torch.randint(0, classes, (rows,), generator=g, device='cuda')
+  advantages, old = torch.randn(2, rows, generator=g, device='cuda').unbind()
+  old = old - 5.0
+  run = lambda a, b: pl.policy_loss(logits[a:b], actions[a:b], advantages[a:b], old[a:b], normalizer=float(rows))
+  whole, cut = run(0, rows), rows // 2 + 5
+  first, last = run(0, cut), run(cut, rows)
+  assert torch.equal(whole.dlogits, torch.cat([first.dlogits, last.dlogits]))
+  assert torch.equal(whole.logp, torch.cat([first.logp, last.logp]))
+  # three roundings to float32 of sums in double
+  big = max(abs(first.loss.item()), abs(last.loss.item()), abs(whole.loss.item()))
+  assert abs(whole.loss.item() - (first.loss.item() + last.loss.item())) <= 4 * U32 * big
+
+
 def test_two_streams_at_once():
   from dqn_zoo_amd import policy_loss as pl
   cfg = pl.PolicyLossConfig(0.2, 0.2, 0.1, 0.02)

@@ -152,7 +152,9 @@ def test_c_entries_refuse(lib):
                  dict(logits=None), dict(actions=None), dict(advantages=None), dict(old_logp=None), dict(logp=None),
                  dict(entropy=None), dict(loss=None), dict(ld=5), dict(ldg=5), dict(clip_low=-0.1),
                  dict(clip_high=-0.1), dict(normalizer=-1.0), dict(ws=4100),
-                 dict(classes=300, ld=300, ldg=300)):   # needs a workspace
+                 dict(classes=300, ld=300, ldg=300),   # needs a workspace
+                 dict(classes=300, ld=300, ldg=300, rows=1 << 26, ws=4096, ws_bytes=1 << 40),   # more threads than
+                 dict(classes=5000, ld=5000, ldg=5000, rows=1 << 24, ws=4096, ws_bytes=1 << 40)):   # a launch has
     assert loss(**change) == bad, change
 
   def adamw(**change):
