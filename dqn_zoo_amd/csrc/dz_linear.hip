@@ -24,7 +24,9 @@ bool readable(const Matrix& x, int64_t elem) {
   const int64_t ve = 16 / elem;
   return x.at && ((uintptr_t)x.at & 15) == 0 && x.ld % ve == 0 && x.cols % ve == 0 && x.ld * elem <= kMaxPitchBytes;
 }
-int64_t packed_ld(const Matrix& x, int64_t elem) { return round_up(x.cols, 16 / elem); }
+// Rows of a copy begin at multiples of 128 bytes: a stage's piece of one would lie in two cache lines
+// otherwise (1777 x 1235 x 1001 fp16: 18.2 -> 15.9 us).
+int64_t packed_ld(const Matrix& x, int64_t elem) { return round_up(x.cols, 128 / elem); }
 int64_t packed_bytes(const Matrix& x, int64_t elem) { return round_up(x.rows * packed_ld(x, elem) * elem, 256); }
 
 // Measured on this card (us; sweeps of tiles and splits over 30 shapes): what a stage of a workgroup

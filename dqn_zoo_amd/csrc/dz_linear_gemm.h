@@ -651,23 +651,31 @@ __global__ __launch_bounds__(64 * kRowsWaves) void linear_rows_any_kernel(DzGemm
 }
 
 // Copies one or two operands into rows of whole 16-byte units, zeros behind their ends: 64 threads
-// along a row, four rows.
+// along a row, four times two rows (4095 x 4095 fp16 alone: one 17.2 us, two 14.9, four 15.0; 1777 x
+// 1235 and 1235 x 1001 together 6.7, 7.0, 7.4).
+constexpr int kPackRows = 2;
 template <typename T>
 __global__ __launch_bounds__(256) void linear_pack_kernel(DzPackArgs p) {
   constexpr int VE = 16 / sizeof(T);
   const DzPackArgs::One q = blockIdx.z ? p.two : p.one;
   const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * VE;
   if (c >= q.cols) return;
-  for (int64_t row = blockIdx.y * 4 + (threadIdx.x >> 6); row < q.rows; row += gridDim.y * 4) {
-    const T* x = (const T*)q.src + row * q.ld + c;
-    DzPack<T, VE> v;
-    if (c + VE <= q.cols) {
-      v = dz_load<T, VE>(x);
-    } else {
+  const bool whole = c + VE <= q.cols;
+  for (int64_t row = blockIdx.y * (4 * kPackRows) + (threadIdx.x >> 6); row < q.rows; row += gridDim.y * (4 * kPackRows)) {
+    DzPack<T, VE> v[kPackRows];
 #pragma unroll
-      for (int e = 0; e < VE; ++e) v.v[e] = c + e < q.cols ? x[e] : (T)0.0f;
+    for (int r = 0; r < kPackRows; ++r) {
+      const T* x = (const T*)q.src + min(row + 4 * r, q.rows - 1) * q.ld + c;
+      if (whole) {
+        v[r] = dz_load<T, VE>(x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) v[r].v[e] = c + e < q.cols ? x[e] : (T)0.0f;
+      }
     }
-    dz_store<T, VE>((T*)q.dst + row * q.ldd + c, v);
+#pragma unroll
+    for (int r = 0; r < kPackRows; ++r)
+      if (row + 4 * r < q.rows) dz_store<T, VE>((T*)q.dst + (row + 4 * r) * q.ldd + c, v[r]);
   }
 }
 

@@ -77,7 +77,7 @@ template <typename T>
 int launch_pack(const DzPackArgs& p, hipStream_t s) {
   constexpr int kCols = 64 * (16 / (int)sizeof(T));
   const int cols = p.one.cols > p.two.cols ? p.one.cols : p.two.cols;
-  int64_t rows = ((p.one.rows > p.two.rows ? p.one.rows : p.two.rows) + 3) / 4;
+  int64_t rows = ((p.one.rows > p.two.rows ? p.one.rows : p.two.rows) + 4 * kPackRows - 1) / (4 * kPackRows);
   if (rows > 65535) rows = 65535;
   const dim3 grid((cols + kCols - 1) / kCols, (unsigned)rows, p.two.src ? 2 : 1);
   hipLaunchKernelGGL((linear_pack_kernel<T>), grid, dim3(256), 0, s, p);
