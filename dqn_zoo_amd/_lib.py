@@ -480,6 +480,22 @@ def new_output(shape, dtype, device):
   return torch.empty(shape, dtype=dtype, device=device)
 
 
+def new_like(t, shape):
+  """`new_output` of t's type and device (half the host's time of a torch.empty with keywords)."""
+  if _raw_capture:
+    return new_output(shape, t.dtype, t.device)
+  import torch
+  return torch.empty_like(t) if t.shape == shape and t.is_contiguous() else t.new_empty(shape)
+
+
+def span(t):
+  """(first, last + 1) byte of a tensor, whatever lies between its rows."""
+  start = t.data_ptr()
+  if t.is_contiguous():
+    return start, start + t.numel() * t.element_size()
+  return start, start + t.element_size() * (1 + sum((s - 1) * d for s, d in zip(t.shape, t.stride())))
+
+
 class _NoGuard:
 
   def __enter__(self):

@@ -75,20 +75,18 @@ def _vector(name, t, n, dtype, device):
   return int(t.dtype == torch.float32)
 
 
-def _span(t):
-  """First and last byte of a matrix, whatever lies between its rows."""
-  start = t.data_ptr()
-  return start, start + t.element_size() * (1 + sum((s - 1) * d for s, d in zip(t.shape, t.stride())))
+def _apart(name, output, taken):
+  """Outputs may not lie on what the kernels still read, or on each other; `output` joins `taken`,
+  a list of (name, first byte, last byte)."""
+  a, b = _lib.span(output)
+  for other, c, d in taken:
+    if a < d and c < b:
+      raise ValueError('%s shares memory with %s' % (name, other))
+  taken.append((name, a, b))
 
 
-def _apart(name, output, **inputs):
-  """Outputs may not lie on what the kernels still read."""
-  a, b = _span(output)
-  for other, t in inputs.items():
-    if t is not None:
-      c, d = _span(t)
-      if a < d and c < b:
-        raise ValueError('%s shares memory with %s' % (name, other))
+def _spans(**tensors):
+  return [(n, *_lib.span(t)) for n, t in tensors.items() if t is not None]
 
 
 def _start(x, w):
@@ -162,20 +160,24 @@ def linear(x: torch.Tensor, w: torch.Tensor, b: typing.Optional[torch.Tensor] = 
   if preact is not None and not save_preact:
     raise ValueError('preact= is a buffer for save_preact=True')
   with _lib.device_guard(device):
+    given = out is not None or preact is not None
+    taken = _spans(x=x, w=w, b=b) if given else None
     if out is None:
-      out = _lib.new_output((m, n), dtype, x.device)
+      out = _lib.new_like(x, (m, n))
       a.ldy = n
     else:
       a.ldy = _rows('out', out, (m, n), dtype, device)
       same = residual is not None and residual.data_ptr() == out.data_ptr() and a.ldr == a.ldy
-      _apart('out', out, x=x, w=w, b=b, residual=None if same else residual)
+      if residual is not None and not same:
+        taken += _spans(residual=residual)
+      _apart('out', out, taken)
     if save_preact:
       if preact is None:
-        preact = _lib.new_output((m, n), dtype, x.device)
+        preact = _lib.new_like(x, (m, n))
         a.ldz = n
       else:
         a.ldz = _rows('preact', preact, (m, n), dtype, device)
-        _apart('preact', preact, x=x, w=w, b=b, residual=residual, out=out)
+        _apart('preact', preact, taken + _spans(residual=residual))
       a.preact = preact.data_ptr()
     a.y = out.data_ptr()
     lib = _lib.load()
@@ -214,15 +216,16 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
   for name, wanted, t in zip(('dx', 'dw', 'db'), need, (dx, dw, db)):
     if t is not None and not wanted:
       raise ValueError('%s= is given but not needed' % name)
-  reads = dict(dy=dy, x=x, w=w, preact=preact)
+  given = dx is not None or dw is not None or db is not None
+  taken = _spans(dy=dy, x=x, w=w, preact=preact) if given else None
   with _lib.device_guard(device):
     if need[0]:
       if dx is None:
-        dx = _lib.new_output((m, k), dtype, x.device)
+        dx = _lib.new_like(x, (m, k))
         a.lddx = k
       else:
         a.lddx = _rows('dx', dx, (m, k), dtype, device)
-        _apart('dx', dx, **reads)
+        _apart('dx', dx, taken)
       a.dx = dx.data_ptr()
     grads = [t for t in (dw, db) if t is not None]
     kind = grads[0].dtype if grads else dtype
@@ -231,20 +234,21 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
     a.grads_f32 = int(kind == torch.float32)
     if need[1]:
       if dw is None:
-        dw = _lib.new_output((n, k) if a.w_transposed else (k, n), kind, x.device)
+        stored = (n, k) if a.w_transposed else (k, n)
+        dw = _lib.new_like(w, stored) if kind == dtype else _lib.new_output(stored, kind, x.device)
         a.lddw = k if a.w_transposed else n
         dw = dw.t() if a.w_transposed else dw
       else:
         a.lddw = _rows('dw, stored as w is,', dw.t() if a.w_transposed else dw,
                        (n, k) if a.w_transposed else (k, n), kind, device)
-        _apart('dw', dw, dx=dx, **reads)
+        _apart('dw', dw, taken)
       a.dw = dw.data_ptr()
     if need[2]:
       if db is None:
-        db = _lib.new_output((n,), kind, x.device)
+        db = _lib.new_like(w, n) if kind == dtype else _lib.new_output((n,), kind, x.device)
       else:
         _vector('db', db, n, dtype, device)
-        _apart('db', db, dx=dx, dw=dw, **reads)
+        _apart('db', db, taken)
       a.db = db.data_ptr()
     lib = _lib.load()
     ws = _workspace(lib, a, 1, x.device, workspace)  # pylint: disable=unused-variable

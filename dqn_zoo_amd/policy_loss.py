@@ -38,6 +38,10 @@ def workspace_bytes(rows: int, classes: int, dtype: torch.dtype) -> int:
   code = _lib.dtype_code(dtype)
   if code is None:
     raise TypeError('logits must be float32, bfloat16 or float16, got %s' % dtype)
+  return _workspace_bytes(code, rows, classes)
+
+
+def _workspace_bytes(code, rows, classes):
   n = ctypes.c_int64()
   _lib.check(_lib.load().dz_policy_loss_workspace(code, rows, classes, ctypes.byref(n)),
              'dz_policy_loss_workspace')
@@ -71,21 +75,21 @@ def _matrix(name, t, shape, dtype, device):
   return max(ld, cols)
 
 
-def _check_apart(out, **inputs):
+def _check_apart(out, logits, **inputs):
   """A row's outputs may be written while another workgroup still reads that row's inputs."""
-  def extent(t):
-    last = sum((s - 1) * d for s, d in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + t.element_size() * (last + 1)
-  outs = [(n, t) for n, t in zip(out._fields, out) if t is not None]
-  for i, (name, t) in enumerate(outs):
-    a, b = extent(t)
-    others = outs[:i] + [(n, x) for n, x in inputs.items() if x is not None]
-    for other, x in others:
-      if other == 'logits' and name == 'dlogits' and x.data_ptr() == a and x.stride() == t.stride():
-        continue
-      c, d = extent(x)
+  taken = [(n, *_lib.span(t)) for n, t in inputs.items() if t is not None]
+  for name, t in zip(out._fields, out):
+    if t is None:
+      continue
+    a, b = _lib.span(t)
+    if not (name == 'dlogits' and logits.data_ptr() == a and logits.stride() == t.stride()):
+      c, d = _lib.span(logits)
+      if a < d and c < b:
+        raise ValueError('out.%s overlaps logits' % name)
+    for other, c, d in taken:
       if a < d and c < b:
         raise ValueError('out.%s overlaps %s' % (name, other))
+    taken.append((name, a, b))
 
 
 def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.Tensor,
@@ -143,10 +147,10 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.T
     a.status = _row_vector('status', status, 1, torch.int32, device)
   with _lib.device_guard(device):
     if out is None:
-      where = logits.device
-      logp, entropy = _lib.new_output((2, rows), f32, where).unbind()
-      out = PolicyLossOutputs(_lib.new_output((), f32, where), logp, entropy,
-                              _lib.new_output(shape, logits.dtype, where) if with_gradient else None)
+      logp, entropy = _lib.new_like(advantages, (2, rows)).unbind()
+      out = PolicyLossOutputs(_lib.new_like(advantages, ()), logp, entropy,
+                              _lib.new_like(logits, shape) if with_gradient else None)
+      a.ldg = classes
     else:
       if _row_vector('out.loss', out.loss.view(1), 1, f32, device) is None or (
           out.dlogits is None) == with_gradient:
@@ -154,20 +158,16 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, advantages: torch.T
       _row_vector('out.logp', out.logp, rows, f32, device)
       _row_vector('out.entropy', out.entropy, rows, f32, device)
       if with_gradient:
-        _matrix('out.dlogits', out.dlogits, shape, logits.dtype, device)
+        a.ldg = _matrix('out.dlogits', out.dlogits, shape, logits.dtype, device)
       _check_apart(out, logits=logits, actions=actions, advantages=advantages, old_logp=old_logp,
                    ref_logp=ref_logp, weights=weights, status=status)
     a.loss, a.logp, a.entropy = out.loss.data_ptr(), out.logp.data_ptr(), out.entropy.data_ptr()
     if with_gradient:
-      g = out.dlogits
-      a.ldg = _matrix('out.dlogits', g, shape, logits.dtype, device)
-      a.dlogits = g.data_ptr()
+      a.dlogits = out.dlogits.data_ptr()
     lib = _lib.load()
-    need = ctypes.c_int64()
-    _lib.check(lib.dz_policy_loss_workspace(code, rows, classes, ctypes.byref(need)),
-               'dz_policy_loss_workspace')
-    if need.value or workspace is not None:
-      ws = _lib.scratch(need.value, logits.device, workspace)
-      a.ws, a.ws_bytes = ws.data_ptr(), need.value
+    need = _workspace_bytes(code, rows, classes)
+    if need or workspace is not None:
+      ws = _lib.scratch(need, logits.device, workspace)
+      a.ws, a.ws_bytes = ws.data_ptr(), need
     _lib.check(lib.dz_policy_loss(ctypes.byref(a), _lib.stream_ptr(device)), 'dz_policy_loss')
   return out
