@@ -136,11 +136,12 @@ Layout plan_backward(const dz_linear_args_t* a) {
   if (l.dx.tile == kRowsAnyTile) l.pack_w = false;
   if (dw) l.dw = a->w_transposed ? plan_gemm(a->n, a->k, a->m, elem, false, false)
                                        : plan_gemm(a->k, a->n, a->m, elem, false, false);
-  // rows of one chunk of the column sums: four workgroups per CU, if the rows allow
+  // rows of one chunk of the column sums: four workgroups per CU, if the rows allow; one chunk for a
+  // batch of 32 (no second launch)
   const int64_t cols = (a->n + 64 * (16 / elem) - 1) / (64 * (16 / elem));
   const int64_t wanted = 4 * kCus / cols < 1 ? 1 : 4 * kCus / cols;
   const int64_t rows = round_up((a->m + wanted - 1) / wanted, 8);
-  l.rows = (int)(rows < 32 ? 32 : rows);
+  l.rows = (int)(a->m <= 32 ? 32 : rows < 16 ? 16 : rows);
   l.chunks = (int)((a->m + l.rows - 1) / l.rows);
   if (l.pack_x) { l.x_at = l.bytes; l.bytes += packed_bytes(x_of(a), elem); }
   if (l.pack_w) { l.w_at = l.bytes; l.bytes += packed_bytes(w_of(a), elem); }
